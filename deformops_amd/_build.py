@@ -1,8 +1,8 @@
 """Ahead-of-time build of the HIP library for gfx950 and of its native torch bridge.
 
-libdeformops_amd.so is the MSDA library (the C ABI of include/deformops_amd.h),
+libdeformops_amd.so holds the kernels (the C ABI of include/deformops_amd.h),
 built in-tree (``deformops_amd/lib/``) with hipcc and loaded with ctypes; _native.so is
-the Python extension module that plain eager calls go through (csrc/bridge.cpp, host
+the Python extension module that plain eager calls go through (csrc/bridge*.cpp, host
 code only). Nothing is compiled at import or call time.
 
     python -m deformops_amd._build
@@ -10,6 +10,7 @@ code only). Nothing is compiled at import or call time.
 
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import shutil
 import subprocess
@@ -22,10 +23,12 @@ __all__ = ["ARCH", "HIPCC_FLAGS", "LIBRARY", "SOURCES", "build", "compile_librar
 
 PACKAGE_DIR = Path(__file__).resolve().parent
 REPO_DIR = PACKAGE_DIR.parent
-SOURCES = [PACKAGE_DIR / "csrc" / "msda.hip"]
+SOURCES = [PACKAGE_DIR / "csrc" / name for name in (
+    "msda.hip", "attention_f32.hip", "attention_f16.hip", "attention_bf16.hip", "attention.hip", "dropout.hip",
+    "rotary.hip")]
 INCLUDE_DIR = REPO_DIR / "include"
 LIBRARY = PACKAGE_DIR / "lib" / "libdeformops_amd.so"
-BRIDGE_SOURCE = PACKAGE_DIR / "csrc" / "bridge.cpp"
+BRIDGE_SOURCES = [PACKAGE_DIR / "csrc" / name for name in ("bridge.cpp", "bridge_operators.cpp")]
 BRIDGE = PACKAGE_DIR / "lib" / "_native.so"
 ARCH = os.environ.get("DEFORMOPS_AMD_ARCH", "gfx950")
 
@@ -53,7 +56,7 @@ def _hipcc() -> str:
 
 
 def build(*, verbose: bool = False) -> Path:
-    """Compile the MSDA library, atomically replacing it; return its path.
+    """Compile the HIP library, atomically replacing it; return its path.
 
     Raises
     ------
@@ -75,7 +78,7 @@ def build_bridge(*, verbose: bool = False) -> Path:
         os.environ.get("CXX") or shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared",
         "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__=1",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",  # noqa: SLF001
-        f"-I{INCLUDE_DIR}", *(f"-isystem{path}" for path in dict.fromkeys(includes)), str(BRIDGE_SOURCE),
+        f"-I{INCLUDE_DIR}", *(f"-isystem{path}" for path in dict.fromkeys(includes)), *map(str, BRIDGE_SOURCES),
         *(f"-L{path}" for path in cpp_extension.library_paths()),
         "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python",
     ]
@@ -83,7 +86,20 @@ def build_bridge(*, verbose: bool = False) -> Path:
 
 
 def compile_library(sources: list[Path], target: Path, *, verbose: bool) -> Path:
-    return _compile([_hipcc(), *HIPCC_FLAGS, *map(str, sources)], target, verbose=verbose)
+    """``sources`` as one shared library; several are compiled side by side and then linked."""
+    command = [_hipcc(), *HIPCC_FLAGS]
+    if len(sources) == 1:
+        return _compile([*command, str(sources[0])], target, verbose=verbose)
+    target.parent.mkdir(parents=True, exist_ok=True)
+    with tempfile.TemporaryDirectory(prefix=target.name + ".", suffix=".tmp", dir=target.parent) as folder:
+        objects = [Path(folder) / f"{source.stem}.o" for source in sources]
+        compiler = [flag for flag in command if flag != "-shared"]
+        with concurrent.futures.ThreadPoolExecutor(min(len(sources), os.cpu_count() or 1, 8)) as pool:
+            jobs = [pool.submit(_compile, [*compiler, "-c", str(source)], built, verbose=verbose)
+                    for source, built in zip(sources, objects)]
+            for job in jobs:
+                job.result()
+        return _compile([*command, *map(str, objects)], target, verbose=verbose)
 
 
 def _compile(command: list[str], target: Path, *, verbose: bool) -> Path:

@@ -69,6 +69,12 @@ EXPORTED_SYMBOLS = (
     "msda_record_plan",
     "msda_set_path_override",
     "msda_set_phase_events",
+    "deformops_cross_attention_workspace_size",
+    "deformops_cross_attention_forward",
+    "deformops_cross_attention_backward",
+    "deformops_rotary",
+    "deformops_dropout",
+    "deformops_last_error",
 )
 
 _P = ctypes.c_void_p
@@ -115,6 +121,18 @@ class Library:
         lib.msda_set_path_override.restype = _I
         lib.msda_set_phase_events.argtypes = [ctypes.POINTER(_P), _I]
         lib.msda_set_phase_events.restype = _I
+        lib.deformops_cross_attention_workspace_size.argtypes = [_P, ctypes.POINTER(_L), ctypes.POINTER(_L)]
+        lib.deformops_cross_attention_workspace_size.restype = _I
+        lib.deformops_cross_attention_forward.argtypes = [_P, _P, _P, _L, _P]
+        lib.deformops_cross_attention_forward.restype = _I
+        lib.deformops_cross_attention_backward.argtypes = [_P, _P, _P, _P, _P, _P, _P, _L, _P]
+        lib.deformops_cross_attention_backward.restype = _I
+        lib.deformops_rotary.argtypes = [_P, _P, _P, _I, _P, _P, _I, _P, _P, *([_L] * 5), _I, _I, _P]
+        lib.deformops_rotary.restype = _I
+        lib.deformops_dropout.argtypes = [_P, _P, _P, _I, _L, ctypes.c_double, ctypes.c_uint64, _P, ctypes.c_uint64, _P]
+        lib.deformops_dropout.restype = _I
+        lib.deformops_last_error.argtypes = []
+        lib.deformops_last_error.restype = ctypes.c_char_p
         self.forward = lib.msda_forward
         self.backward = lib.msda_backward
         self.backward_workspace = lib.msda_backward_workspace

@@ -1,4 +1,4 @@
-"""The native bridge of plain eager calls (csrc/bridge.cpp), loaded on first use.
+"""The native bridge of plain eager calls (csrc/bridge*.cpp), loaded on first use.
 
 ``deformops_amd/lib/_native.so`` is a Python extension module built with the HIP
 library (``python -m deformops_amd._build``); it calls that library's entry points at
@@ -75,5 +75,9 @@ def load(*, download: bool | None = None, compile: bool | str | None = None) -> 
         entry_points = (library.cdll.msda_forward, library.cdll.msda_backward_workspace,
                         library.cdll.msda_backward_workspace_size, library.cdll.msda_last_error)
         module.init(*(ctypes.cast(f, ctypes.c_void_p).value for f in entry_points))
+        operators = (library.cdll.deformops_cross_attention_workspace_size,
+                     library.cdll.deformops_cross_attention_forward, library.cdll.deformops_cross_attention_backward,
+                     library.cdll.deformops_rotary, library.cdll.deformops_dropout, library.cdll.deformops_last_error)
+        module.init_operators([ctypes.cast(f, ctypes.c_void_p).value for f in operators])
         _loaded = module
         return module

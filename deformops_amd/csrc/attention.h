@@ -1,0 +1,1105 @@
+// Cross attention (softmax(scale q k^T + mask) v) for gfx950, forward and backward, behind
+// deformops_cross_attention_* of include/deformops_amd.h.
+//
+// Mathematics. With x_ij the scaled and masked score of row i and key j, m_i = max_j x_ij:
+//   p_ij = exp(x_ij - m_i) / l_i,   l_i = sum_j exp(x_ij - m_i),   o_i = sum_j p_ij v_j
+//   dv_j = sum_i p_ij do_i,   ds_ij = p_ij (do_i . v_j - delta_i),   delta_i = do_i . o_i
+//   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i
+// The forward passes over the keys once with a running maximum and sum, and keeps (m, log2 l)
+// of each row, from which the backward forms p again. A row that no key is left for has o = 0
+// and no gradient: its m is kept as +inf, which makes every p of it 0.
+//
+// Rows. The heads that share a key head are one list of rows: row r of (image, key head) is
+// query r / G of head r % G in the group, G = heads / key heads. So the states are read once
+// for the whole group, a group's gradients of k and v are summed in one place, and a single
+// token's G heads fill one tile.
+//
+// Products. All run on v_mfma_f32_32x32x16_{bf16,f16} or v_mfma_f32_32x32x2_f32, whose result
+// has column = lane % 32 and rows 8 (r / 4) + 4 (lane / 32) + r % 4 in its 16 registers. The
+// scores are formed so that the axis of the next product's contraction lies in the registers:
+// keys x rows for o and dq, rows x keys for dv and dk. A product contracts over its axis in
+// any order as long as both operands agree, so the registers are the next product's operand
+// as they are, and the other operand is read from LDS in the registers' order
+// (ds_read_b64_tr_b16 turns a row-major 16-bit tile on the way). Scores never touch LDS, and a
+// softmax statistic of the keys x rows form is one value per lane.
+
+#ifndef DEFORMOPS_AMD_ATTENTION_H_
+#define DEFORMOPS_AMD_ATTENTION_H_
+
+#include <algorithm>
+#include <math.h>
+#include <type_traits>
+
+#include "operators.h"
+
+namespace attention {
+
+using namespace operators;
+
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
+typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -INFINITY;
+
+enum MaskKind { kNoMask = 0, kBoolMask = 1, kFloatMask = 2 };
+
+struct Args {
+  const void *q, *k, *v;
+  int64_t q_batch, q_row, q_head, k_batch, k_row, k_head, v_batch, v_row, v_head;
+  const void* mask;
+  int64_t mask_batch, mask_head, mask_row, mask_key;
+  int mask_type;    // element type of a float mask
+  bool mask_quads;  // four keys of a row lie side by side, aligned to their size
+  bool mask_of_keys;  // a bool mask that is one for all rows and heads: it removes states
+  const void* lengths;
+  bool lengths_i64;
+  void* out;
+  float2* stats;  // (m, log2 l) of each row, m = +inf for a row without keys
+  int B, Q, S, K, G, D;
+  uint32_t R;  // rows of one (image, key head): Q * G
+  float scale;
+  bool vector;  // operand rows may be read in 16-byte pieces
+  bool out_vector;
+  int splits;
+  float* part;         // [splits][B * K][R][D] unnormalized sums of each split
+  float2* part_stats;  // [splits][B * K][R]
+  // Backward.
+  const void* grad_out;
+  const float2* row_stats;
+  float* delta;  // [B * K][R]
+  void *grad_q, *grad_k, *grad_v;
+  int row_splits;
+  float* part_k;  // [row_splits][B][S][K][D]
+  float* part_v;
+};
+
+// ---------------------------------------------------------------------------
+// Matrix products of one wave.
+
+// Precision of a 16-bit operand made from fp32 scores: p and ds are rounded to the operands'
+// type (bf16 2^-9, f16 2^-12 relative). f16 has 5 exponent bits: p is scaled by 2^14, so
+// that weights down to 2^-28 stay normal, and ds by a running power of two for each lane
+// (Scaled below).
+template <typename T> constexpr float kWeightBits = std::is_same_v<T, f16_t> ? 14.0f : 0.0f;
+
+template <typename T> struct Mma;
+
+template <typename T> struct Mma16 {
+  using Vec = std::conditional_t<std::is_same_v<T, bf16_t>, bf16x8, f16x8>;
+  struct Weights { Vec part[2]; };  // 32 contracted positions
+
+  static __device__ f32x16 mma(Vec a, Vec b, f32x16 c) {
+    if constexpr (std::is_same_v<T, bf16_t>)
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  // One 16-byte piece of 32 rows of each operand: 16 contracted channels.
+  static __device__ f32x16 rows(u32x4 a, u32x4 b, f32x16 c) {
+    return mma(__builtin_bit_cast(Vec, a), __builtin_bit_cast(Vec, b), c);
+  }
+  static __device__ Weights weights(const float (&w)[16]) {
+    Weights out;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) out.part[i / 8][i % 8] = static_cast<T>(w[i]);
+    return out;
+  }
+};
+template <> struct Mma<bf16_t> : Mma16<bf16_t> {};
+template <> struct Mma<f16_t> : Mma16<f16_t> {};
+template <> struct Mma<float> {
+  struct Weights { float part[16]; };
+  static __device__ f32x16 rows(u32x4 a, u32x4 b, f32x16 c) {
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[i], c, 0, 0, 0);
+    return c;
+  }
+  static __device__ Weights weights(const float (&w)[16]) {
+    Weights out;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) out.part[i] = w[i];
+    return out;
+  }
+};
+
+// A tile of rows in LDS, DP channels each, in 16-byte pieces. The pieces of a row change
+// places by an exclusive or with the row's number, so that neighbouring rows' equal pieces
+// lie in different banks.
+template <typename T, int DP> struct Tile {
+  static constexpr int kPieces = DP * int(sizeof(T)) / 16;
+  static constexpr int kRowBytes = kPieces * 16;
+
+  static __device__ int offset(int row, int piece) {
+    int turn;
+    if constexpr (kPieces % 8 == 0)
+      turn = row & 7;
+    else if constexpr (kPieces == 4)
+      turn = (row >> 1) & 3;
+    else
+      turn = (row >> 2) & 3;
+    return row * kRowBytes + ((piece ^ turn) << 4);
+  }
+};
+
+// acc (channels x lanes) += tile^T (32 channels from 32 * block, the 32 tile rows from `row`)
+// x w: the sum over tile rows of w[row][lane] * tile[row][channel].
+template <typename T, int DP>
+__device__ inline f32x16 accumulate(const char* tile, int row, int block, const typename Mma<T>::Weights& w,
+                                    f32x16 acc) {
+  const int lane = threadIdx.x % kWave, half = lane / 32;
+  if constexpr (sizeof(T) == 2) {
+    // Lane c of a 16-lane group gets channel c of the four rows that the group reads.
+    const int channel = 32 * block + 16 * ((lane / 16) & 1) + 4 * (lane % 4);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      i16x4 part[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int r = row + 16 * t + 8 * u + 4 * half + (lane % 16) / 4;
+        const char* at = tile + Tile<T, DP>::offset(r, channel / 8) + (channel % 8) * 2;
+        part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) i16x4*)(at));
+      }
+      const i16x8 both = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      acc = Mma<T>::mma(__builtin_bit_cast(typename Mma<T>::Vec, both), w.part[t], acc);
+    }
+  } else {
+    const int channel = 32 * block + lane % 32;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = row + 8 * (i / 4) + 4 * half + i % 4;
+      const float a = *reinterpret_cast<const float*>(tile + Tile<T, DP>::offset(r, channel / 4) + (channel % 4) * 4);
+      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a, w.part[i], acc, 0, 0, 0);
+    }
+  }
+  return acc;
+}
+
+// The product's row operand: piece 2 * step + half of tile row `row + lane % 32`.
+template <typename T, int DP> __device__ inline u32x4 row_piece(const char* tile, int row, int step) {
+  const int lane = threadIdx.x % kWave;
+  return *reinterpret_cast<const u32x4*>(tile + Tile<T, DP>::offset(row + lane % 32, 2 * step + lane / 32));
+}
+
+// 16 bytes of a row in memory, from channel c; zero past D.
+template <typename T> __device__ inline u32x4 load_piece(const T* row, int c, int D, bool vector) {
+  constexpr int N = 16 / int(sizeof(T));
+  u32x4 out = {0, 0, 0, 0};
+  if (vector) {  // then D is a multiple of N
+    if (c < D) out = *reinterpret_cast<const u32x4*>(row + c);
+    return out;
+  }
+  T parts[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) parts[i] = c + i < D ? row[c + i] : T(0);
+  __builtin_memcpy(&out, parts, 16);
+  return out;
+}
+
+// The largest of a lane's value and its partner's, 32 lanes on.
+__device__ inline float half_max(float v) {
+  const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+__device__ inline float half_sum(float v) {
+  const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(both[0]) + __uint_as_float(both[1]);
+}
+
+// The keys' (or rows') number in a 32 x 32 result's register r.
+__device__ inline int result_row(int r) { return 8 * (r / 4) + 4 * ((threadIdx.x % kWave) / 32) + r % 4; }
+
+// f16 only: ds as operands of the matrix cores, scaled by a power of two for each lane. ds
+// spans what p and the incoming gradient span together (p alone reaches 1e-6 at 2^20 keys),
+// more than f16's 2^-24 .. 2^16 in ordinary training. A lane's ds all go into sums that the
+// lane's column holds, so each lane keeps an exponent of its own, taken from the first values
+// (to 2^11 .. 2^12) and lowered, with the sums so far, when a later value would pass 2^15.
+template <typename T> struct Scaled {
+  template <int N> __device__ void fit(float (&)[16], f32x16 (&)[N]) {}
+  __device__ float undo(float v) const { return v; }
+};
+template <> struct Scaled<f16_t> {
+  int e = 1 << 20;  // none yet
+  template <int N> __device__ void fit(float (&ds)[16], f32x16 (&acc)[N]) {
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(ds[i]));
+    top = half_max(top);
+    int bits = __builtin_amdgcn_frexp_expf(top);  // top = f 2^bits, f in [0.5, 1); 0 for 0, inf and NaN
+    const bool change = top > 0.0f && bits + e > 15;
+    if (__any(change)) {
+      const int next = change ? min(12 - bits, 120) : e;
+      const int by = e == (1 << 20) ? 0 : next - e;  // the sums are zero before the first
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[n][i] = ldexpf(acc[n][i], by);
+      e = next;
+    }
+    const int by = e == (1 << 20) ? 0 : e;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) ds[i] = ldexpf(ds[i], by);
+  }
+  __device__ float undo(float v) const { return ldexpf(v, e == (1 << 20) ? 0 : -e); }
+};
+
+// ---------------------------------------------------------------------------
+// Masks and lengths.
+
+__device__ inline int states_of(const Args& a, int b) {
+  if (!a.lengths) return a.S;
+  const int64_t n = a.lengths_i64 ? static_cast<const int64_t*>(a.lengths)[b]
+                                  : int64_t(static_cast<const int32_t*>(a.lengths)[b]);
+  return int(n < 0 ? 0 : n > a.S ? a.S : n);
+}
+
+__device__ inline float float_mask(const Args& a, int64_t at) {
+  if (a.mask_type == MSDA_F32) return static_cast<const float*>(a.mask)[at];
+  if (a.mask_type == MSDA_BF16) return widen(static_cast<const bf16_t*>(a.mask)[at]);
+  return widen(static_cast<const f16_t*>(a.mask)[at]);
+}
+__device__ inline bool bool_mask(const Args& a, int64_t at) { return static_cast<const uint8_t*>(a.mask)[at] != 0; }
+
+// Bit r: whether the mask leaves the key of result row r (32 keys from `key`) to the row whose
+// first mask element is `at`. Keys at or past `limit` count as left out.
+__device__ inline uint32_t bool_bits(const Args& a, int64_t at, int key, int limit) {
+  uint32_t bits = 0;
+  const int half = (threadIdx.x % kWave) / 32;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int k0 = key + 8 * g + 4 * half;
+    if (a.mask_quads && k0 + 4 <= limit) {
+      const uint32_t four = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.mask) + at + k0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bits |= uint32_t(((four >> (8 * i)) & 0xff) != 0) << (4 * g + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (k0 + i < limit) bits |= uint32_t(bool_mask(a, at + int64_t(k0 + i) * a.mask_key)) << (4 * g + i);
+    }
+  }
+  return bits;
+}
+
+// The additive mask of the 16 result rows, -inf at or past `limit`.
+__device__ inline void float_masks(const Args& a, int64_t at, int key, int limit, float (&out)[16]) {
+  const int half = (threadIdx.x % kWave) / 32;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int k0 = key + 8 * g + 4 * half;
+    if (a.mask_quads && k0 + 4 <= limit && a.mask_type == MSDA_F32) {
+      const f32x4 four = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.mask) + at + k0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out[4 * g + i] = four[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        out[4 * g + i] = k0 + i < limit ? float_mask(a, at + int64_t(k0 + i) * a.mask_key) : kLowest;
+    }
+  }
+}
+
+// Rows of a (image, key head): query and head of row r.
+struct RowOf {
+  int query, head;
+};
+__device__ inline RowOf row_of(const Args& a, int kv, uint32_t r) {
+  const uint32_t q = a.G == 1 ? r : r / uint32_t(a.G);
+  return RowOf{int(q), kv * a.G + int(r - q * uint32_t(a.G))};
+}
+
+__device__ inline int64_t mask_row_at(const Args& a, int b, RowOf o) {
+  return b * a.mask_batch + int64_t(o.head) * a.mask_head + int64_t(o.query) * a.mask_row;
+}
+
+// ---------------------------------------------------------------------------
+// Staging: tile rows from memory to LDS through registers, so that the next tile's loads are
+// under way while this one is worked on.
+
+template <typename T, int DP, int ROWS, int THREADS> struct Stage {
+  static constexpr int kPieces = Tile<T, DP>::kPieces;
+  static constexpr int kEach = ROWS * kPieces / THREADS;
+  static_assert(ROWS * kPieces % THREADS == 0);
+  static constexpr int kBytes = ROWS * Tile<T, DP>::kRowBytes;
+  u32x4 hold[kEach];
+
+  // `row_at(row)` is the row's address, or null for a row of zeros.
+  template <typename F> __device__ void load(F row_at, int D, bool vector) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int n = i * THREADS + int(threadIdx.x), row = n / kPieces, piece = n % kPieces;
+      const T* p = row_at(row);
+      const u32x4 zero = {0, 0, 0, 0};
+      hold[i] = p ? load_piece(p, piece * (16 / int(sizeof(T))), D, vector) : zero;
+    }
+  }
+  __device__ void store(char* tile) const {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int n = i * THREADS + int(threadIdx.x);
+      *reinterpret_cast<u32x4*>(tile + Tile<T, DP>::offset(n / kPieces, n % kPieces)) = hold[i];
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Forward. A workgroup has 4 waves: WR of them along the rows (32 each), 4 / WR along the keys
+// of a tile (KB blocks of 32 each), whose partial sums meet in LDS at the end. Splits of the
+// key axis leave unnormalized sums, which combine_kernel joins.
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+
+template <typename T, int DP, int WR> struct ForwardShape {
+  static constexpr int WK = kWaves / WR;
+  static constexpr int KB = WR == kWaves ? 2 : 1;
+  static constexpr int kRows = 32 * WR;
+  static constexpr int kKeys = 32 * KB * WK;
+  static constexpr int kTile = kKeys * Tile<T, DP>::kRowBytes;
+  static constexpr int kBuffers = 4 * kTile <= 128 * 1024 ? 2 : 1;
+  static constexpr int kJoin = WK > 1 ? WK * 32 * WR * (DP + 2) * 4 : 0;
+  static constexpr int kLds = std::max(2 * kBuffers * kTile, kJoin);
+};
+
+// Four consecutive channels of a result, rounded to T.
+template <typename T> __device__ inline void store_four(T* p, const float (&v)[4], int left, bool vector) {
+  if (vector && left >= 4) {
+    T parts[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) parts[i] = static_cast<T>(v[i]);
+    if constexpr (sizeof(T) == 2) {
+      u32x2 w;
+      __builtin_memcpy(&w, parts, 8);
+      *reinterpret_cast<u32x2*>(p) = w;
+    } else {
+      u32x4 w;
+      __builtin_memcpy(&w, parts, 16);
+      *reinterpret_cast<u32x4*>(p) = w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < left) p[i] = static_cast<T>(v[i]);
+}
+
+// The running softmax of one row in each lane, over keys x rows results.
+template <int NB> struct Softmax {
+  float m = kLowest;  // in log2 units without a float mask, natural ones with it
+  float l = 0.0f;     // this half's keys only
+  f32x16 acc[NB] = {};
+
+  __device__ void rescale(float factor) {
+    l *= factor;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[n][i] *= factor;
+  }
+};
+
+template <typename T, int DP, int MASK, int WR>
+__global__ __launch_bounds__(kThreads) void attention_forward_kernel(const Args a) {
+  using Shape = ForwardShape<T, DP, WR>;
+  using TileT = Tile<T, DP>;
+  constexpr int KB = Shape::KB, NB = DP / 32, kSteps = TileT::kPieces / 2, kKeys = Shape::kKeys;
+  __shared__ __attribute__((aligned(16))) char lds[Shape::kLds];
+
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int wr = wave % WR, wk = wave / WR;
+  const uint32_t row_tiles = (a.R + Shape::kRows - 1) / Shape::kRows;
+  uint32_t id = xcd_order(blockIdx.x, gridDim.x);
+  const uint32_t row_tile = id % row_tiles;
+  id /= row_tiles;
+  const int split = int(id % uint32_t(a.splits));
+  const int bk = int(id / uint32_t(a.splits));
+  const int b = bk / a.K, kv = bk % a.K;
+
+  const uint32_t r = row_tile * Shape::kRows + 32 * wr + lane % 32;
+  const bool live = r < a.R;
+  const RowOf mine = row_of(a, kv, live ? r : a.R - 1);
+
+  u32x4 q[kSteps];
+  {
+    const T* row = static_cast<const T*>(a.q) + b * a.q_batch + int64_t(mine.query) * a.q_row + mine.head * a.q_head;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const u32x4 zero = {0, 0, 0, 0};
+      q[s] = live ? load_piece(row, (2 * s + lane / 32) * (16 / int(sizeof(T))), a.D, a.vector) : zero;
+    }
+  }
+  int64_t mask_at = 0;
+  if constexpr (MASK != kNoMask) mask_at = mask_row_at(a, b, mine);
+
+  // This split's keys: whole tiles of this image's states.
+  const int states = states_of(a, b);
+  const int tiles = (states + kKeys - 1) / kKeys;
+  const int first = int(int64_t(tiles) * split / a.splits), last = int(int64_t(tiles) * (split + 1) / a.splits);
+
+  const T* k_base = static_cast<const T*>(a.k) + b * a.k_batch + kv * a.k_head;
+  const T* v_base = static_cast<const T*>(a.v) + b * a.v_batch + kv * a.v_head;
+  auto kept = [&](int key) {  // a state that the lengths or a mask of keys removes is read as zero
+    if (key >= states) return false;
+    if constexpr (MASK == kBoolMask)
+      if (a.mask_of_keys) return bool_mask(a, b * a.mask_batch + int64_t(key) * a.mask_key);
+    return true;
+  };
+  Stage<T, DP, kKeys, kThreads> k_stage, v_stage;
+  auto load = [&](int tile) {
+    k_stage.load([&](int row) -> const T* {
+      const int key = tile * kKeys + row;
+      return kept(key) ? k_base + int64_t(key) * a.k_row : nullptr;
+    }, a.D, a.vector);
+    v_stage.load([&](int row) -> const T* {
+      const int key = tile * kKeys + row;
+      return kept(key) ? v_base + int64_t(key) * a.v_row : nullptr;
+    }, a.D, a.vector);
+  };
+
+  Softmax<NB> soft;
+  const float factor = MASK == kFloatMask ? a.scale : a.scale * kLog2e;
+  if (first < last) load(first);
+  for (int tile = first; tile < last; ++tile) {
+    char* k_tile = lds + ((tile - first) % Shape::kBuffers) * 2 * Shape::kTile;
+    char* v_tile = k_tile + Shape::kTile;
+    if (Shape::kBuffers == 1 && tile > first) __syncthreads();
+    k_stage.store(k_tile);
+    v_stage.store(v_tile);
+    __syncthreads();
+    if (tile + 1 < last) load(tile + 1);
+
+    const int key0 = tile * kKeys + 32 * KB * wk;  // this wave's keys
+    const int local = 32 * KB * wk;
+    uint32_t bits[KB];
+    if constexpr (MASK == kBoolMask) {
+      uint32_t any = 0;
+#pragma unroll
+      for (int n = 0; n < KB; ++n) any |= bits[n] = bool_bits(a, mask_at, key0 + 32 * n, states);
+      if (!__any(any != 0 && live)) continue;
+    }
+    float x[KB][16];
+#pragma unroll
+    for (int n = 0; n < KB; ++n) {
+      f32x16 s = {};
+#pragma unroll
+      for (int t = 0; t < kSteps; ++t) s = Mma<T>::rows(row_piece<T, DP>(k_tile, local + 32 * n, t), q[t], s);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[n][i] = s[i];
+    }
+    if constexpr (MASK == kBoolMask) {
+#pragma unroll
+      for (int n = 0; n < KB; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[n][i] = (bits[n] >> i) & 1 ? x[n][i] : kLowest;
+    } else if constexpr (MASK == kFloatMask) {
+#pragma unroll
+      for (int n = 0; n < KB; ++n) {
+        float add[16];
+        float_masks(a, mask_at, key0 + 32 * n, states, add);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[n][i] = add[i] == kLowest ? kLowest : fmaf(x[n][i], factor, add[i]);
+      }
+    } else if (key0 + 32 * KB > states) {
+#pragma unroll
+      for (int n = 0; n < KB; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[n][i] = key0 + 32 * n + result_row(i) < states ? x[n][i] : kLowest;
+    }
+    float top = kLowest;
+#pragma unroll
+    for (int n = 0; n < KB; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, x[n][i]);
+    top = half_max(top);
+    if constexpr (MASK != kFloatMask) top *= factor;
+    if (__any(top > soft.m)) {
+      const float m = fmaxf(soft.m, top);
+      const float by = m == soft.m ? 0.0f : soft.m - m;  // 0 too where both are -inf
+      soft.rescale(__builtin_amdgcn_exp2f(MASK == kFloatMask ? by * kLog2e : by));
+      soft.m = m;
+    }
+    const float base = soft.m == kLowest ? 0.0f : soft.m;  // all -inf: every weight is exp2(-inf)
+    float sum = 0.0f;
+#pragma unroll
+    for (int n = 0; n < KB; ++n) {
+      float p[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float y = MASK == kFloatMask ? fmaf(x[n][i] - base, kLog2e, kWeightBits<T>)
+                                           : fmaf(x[n][i], factor, kWeightBits<T> - base);
+        p[i] = __builtin_amdgcn_exp2f(y);
+        sum += p[i];
+      }
+      const auto w = Mma<T>::weights(p);
+#pragma unroll
+      for (int c = 0; c < NB; ++c) soft.acc[c] = accumulate<T, DP>(v_tile, local + 32 * n, c, w, soft.acc[c]);
+    }
+    soft.l += sum;
+  }
+
+  // Join the waves that share rows: each leaves its sums in LDS, wave 0 of them adds.
+  soft.l = half_sum(soft.l);
+  if constexpr (Shape::WK > 1) {
+    __syncthreads();
+    float* mine_at = reinterpret_cast<float*>(lds) + wave * 32 * (DP + 2);
+    if (lane < 32) {
+      mine_at[32 * DP + lane] = soft.m;
+      mine_at[32 * DP + 32 + lane] = soft.l;
+    }
+#pragma unroll
+    for (int c = 0; c < NB; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mine_at[(32 * c + result_row(i)) * 32 + lane % 32] = soft.acc[c][i];
+    __syncthreads();
+    if (wk > 0) return;
+    for (int other = 1; other < Shape::WK; ++other) {
+      const float* at = reinterpret_cast<const float*>(lds) + (other * WR + wr) * 32 * (DP + 2);
+      const float m2 = at[32 * DP + lane % 32], l2 = at[32 * DP + 32 + lane % 32];
+      const float m = fmaxf(soft.m, m2);
+      const float unit = MASK == kFloatMask ? kLog2e : 1.0f;
+      const float f1 = m == soft.m ? 1.0f : __builtin_amdgcn_exp2f((soft.m - m) * unit);
+      const float f2 = m == m2 ? 1.0f : __builtin_amdgcn_exp2f((m2 - m) * unit);
+      soft.rescale(f1);
+      soft.m = m;
+      soft.l = fmaf(l2, f2, soft.l);
+#pragma unroll
+      for (int c = 0; c < NB; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          soft.acc[c][i] = fmaf(at[(32 * c + result_row(i)) * 32 + lane % 32], f2, soft.acc[c][i]);
+    }
+  }
+  if (!live) return;
+
+  if (a.splits > 1) {
+    const int64_t at = (int64_t(split) * a.B * a.K + bk) * a.R + r;
+    if (lane < 32) a.part_stats[at] = float2{soft.m, soft.l};
+    float* part = a.part + at * a.D;
+#pragma unroll
+    for (int c = 0; c < NB; ++c)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * c + 8 * g + 4 * (lane / 32);
+        const float v[4] = {soft.acc[c][4 * g], soft.acc[c][4 * g + 1], soft.acc[c][4 * g + 2], soft.acc[c][4 * g + 3]};
+        store_four(part + d, v, a.D - d, a.D % 4 == 0);
+      }
+    return;
+  }
+  const float inverse = soft.m == kLowest ? 0.0f : 1.0f / soft.l;
+  if (a.stats && lane < 32)
+    a.stats[int64_t(bk) * a.R + r] = soft.m == kLowest ? float2{INFINITY, 0.0f}
+                                                       : float2{soft.m, log2f(soft.l) - kWeightBits<T>};
+  T* out = static_cast<T*>(a.out) + ((int64_t(b) * a.Q + mine.query) * (a.K * a.G) + mine.head) * a.D;
+#pragma unroll
+  for (int c = 0; c < NB; ++c)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * c + 8 * g + 4 * (lane / 32);
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = soft.acc[c][4 * g + i] * inverse;
+      store_four(out + d, v, a.D - d, a.out_vector);
+    }
+}
+
+// Joins the splits of the forward: one thread per row and four channels.
+template <typename T> __global__ __launch_bounds__(256) void attention_combine_kernel(const Args a, bool natural) {
+  const int quads = (a.D + 3) / 4;
+  const int64_t rows = int64_t(a.B) * a.K * a.R;
+  const int64_t n = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (n >= rows * quads) return;
+  const int64_t row = n / quads;
+  const int d = int(n % quads) * 4;
+  const float unit = natural ? kLog2e : 1.0f;
+  float m = kLowest;
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_stats[s * rows + row].x);
+  float l = 0.0f, v[4] = {};
+  const int left = a.D - d;
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 st = a.part_stats[s * rows + row];
+    if (st.x == kLowest) continue;
+    const float f = st.x == m ? 1.0f : __builtin_amdgcn_exp2f((st.x - m) * unit);
+    l = fmaf(st.y, f, l);
+    const float* p = a.part + (s * rows + row) * a.D + d;
+    if (a.D % 4 == 0) {
+      const f32x4 four = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = fmaf(four[i], f, v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < left) v[i] = fmaf(p[i], f, v[i]);
+    }
+  }
+  const float inverse = m == kLowest ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] *= inverse;
+  const int bk = int(row / a.R), b = bk / a.K;
+  const RowOf o = row_of(a, bk % a.K, uint32_t(row % a.R));
+  T* out = static_cast<T*>(a.out) + ((int64_t(b) * a.Q + o.query) * (a.K * a.G) + o.head) * a.D;
+  store_four(out + d, v, left, a.out_vector);
+  if (a.stats && d == 0)
+    a.stats[row] = m == kLowest ? float2{INFINITY, 0.0f} : float2{m, log2f(l) - kWeightBits<T>};
+}
+
+// ---------------------------------------------------------------------------
+// Backward, queries: the forward's walk over the keys with p formed from the row's statistics.
+// It also leaves delta_i = do_i . o_i of its rows for the states' kernel.
+
+template <typename T, int DP, int MASK, int WR>
+__global__ __launch_bounds__(kThreads) void attention_grad_q_kernel(const Args a) {
+  using Shape = ForwardShape<T, DP, WR>;
+  using TileT = Tile<T, DP>;
+  constexpr int KB = Shape::KB, NB = DP / 32, kSteps = TileT::kPieces / 2, kKeys = Shape::kKeys;
+  constexpr int N = 16 / int(sizeof(T));
+  __shared__ __attribute__((aligned(16))) char lds[Shape::kLds];
+
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int wr = wave % WR, wk = wave / WR;
+  const uint32_t row_tiles = (a.R + Shape::kRows - 1) / Shape::kRows;
+  uint32_t id = xcd_order(blockIdx.x, gridDim.x);
+  const uint32_t row_tile = id % row_tiles;
+  id /= row_tiles;
+  const int split = int(id % uint32_t(a.splits));
+  const int bk = int(id / uint32_t(a.splits));
+  const int b = bk / a.K, kv = bk % a.K;
+
+  const uint32_t r = row_tile * Shape::kRows + 32 * wr + lane % 32;
+  const bool live = r < a.R;
+  const RowOf mine = row_of(a, kv, live ? r : a.R - 1);
+  const int64_t out_at = ((int64_t(b) * a.Q + mine.query) * (a.K * a.G) + mine.head) * a.D;
+
+  u32x4 q[kSteps], go[kSteps];
+  float delta = 0.0f;
+  {
+    const T* row = static_cast<const T*>(a.q) + b * a.q_batch + int64_t(mine.query) * a.q_row + mine.head * a.q_head;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int c = (2 * s + lane / 32) * N;
+      const u32x4 zero = {0, 0, 0, 0};
+      q[s] = live ? load_piece(row, c, a.D, a.vector) : zero;
+      go[s] = live ? load_piece(static_cast<const T*>(a.grad_out) + out_at, c, a.D, a.out_vector) : zero;
+      const u32x4 o = live ? load_piece(static_cast<const T*>(a.out) + out_at, c, a.D, a.out_vector) : zero;
+      T x[N], y[N];
+      __builtin_memcpy(x, &go[s], 16);
+      __builtin_memcpy(y, &o, 16);
+#pragma unroll
+      for (int i = 0; i < N; ++i) delta = fmaf(widen(x[i]), widen(y[i]), delta);
+    }
+    delta = half_sum(delta);
+  }
+  const float2 stat = live ? a.row_stats[int64_t(bk) * a.R + r] : float2{INFINITY, 0.0f};
+  if (split == 0 && wk == 0 && live && lane < 32) a.delta[int64_t(bk) * a.R + r] = delta;
+  int64_t mask_at = 0;
+  if constexpr (MASK != kNoMask) mask_at = mask_row_at(a, b, mine);
+
+  const int states = states_of(a, b);
+  const int tiles = (states + kKeys - 1) / kKeys;
+  const int first = int(int64_t(tiles) * split / a.splits), last = int(int64_t(tiles) * (split + 1) / a.splits);
+  const T* k_base = static_cast<const T*>(a.k) + b * a.k_batch + kv * a.k_head;
+  const T* v_base = static_cast<const T*>(a.v) + b * a.v_batch + kv * a.v_head;
+  auto kept = [&](int key) {
+    if (key >= states) return false;
+    if constexpr (MASK == kBoolMask)
+      if (a.mask_of_keys) return bool_mask(a, b * a.mask_batch + int64_t(key) * a.mask_key);
+    return true;
+  };
+  Stage<T, DP, kKeys, kThreads> k_stage, v_stage;
+  auto load = [&](int tile) {
+    k_stage.load([&](int row) -> const T* {
+      const int key = tile * kKeys + row;
+      return kept(key) ? k_base + int64_t(key) * a.k_row : nullptr;
+    }, a.D, a.vector);
+    v_stage.load([&](int row) -> const T* {
+      const int key = tile * kKeys + row;
+      return kept(key) ? v_base + int64_t(key) * a.v_row : nullptr;
+    }, a.D, a.vector);
+  };
+
+  f32x16 acc[NB] = {};
+  Scaled<T> scaled;
+  const float factor = MASK == kFloatMask ? a.scale : a.scale * kLog2e;
+  const float shift = kWeightBits<T> - (MASK == kFloatMask ? stat.y : stat.x + stat.y);
+  if (first < last) load(first);
+  for (int tile = first; tile < last; ++tile) {
+    char* k_tile = lds + ((tile - first) % Shape::kBuffers) * 2 * Shape::kTile;
+    char* v_tile = k_tile + Shape::kTile;
+    if (Shape::kBuffers == 1 && tile > first) __syncthreads();
+    k_stage.store(k_tile);
+    v_stage.store(v_tile);
+    __syncthreads();
+    if (tile + 1 < last) load(tile + 1);
+
+#pragma unroll
+    for (int n = 0; n < KB; ++n) {
+      const int local = 32 * (KB * wk + n), key0 = tile * kKeys + local;
+      uint32_t bits = 0;
+      if constexpr (MASK == kBoolMask) {
+        bits = bool_bits(a, mask_at, key0, states);
+        if (!__any(bits != 0 && live)) continue;
+      }
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int t = 0; t < kSteps; ++t) {
+        s = Mma<T>::rows(row_piece<T, DP>(k_tile, local, t), q[t], s);
+        dp = Mma<T>::rows(row_piece<T, DP>(v_tile, local, t), go[t], dp);
+      }
+      float ds[16], add[16];
+      if constexpr (MASK == kFloatMask) float_masks(a, mask_at, key0, states, add);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        bool on = true;
+        float y;
+        if constexpr (MASK == kFloatMask) {
+          on = add[i] != kLowest;
+          y = fmaf(fmaf(s[i], factor, add[i]) - stat.x, kLog2e, shift);
+        } else {
+          if constexpr (MASK == kBoolMask) on = (bits >> i) & 1;
+          else on = key0 + result_row(i) < states;
+          y = fmaf(s[i], factor, shift);
+        }
+        const float p = __builtin_amdgcn_exp2f(y);
+        ds[i] = on ? p * (dp[i] - delta) : 0.0f;
+      }
+      scaled.fit(ds, acc);
+      const auto w = Mma<T>::weights(ds);
+#pragma unroll
+      for (int c = 0; c < NB; ++c) acc[c] = accumulate<T, DP>(k_tile, local, c, w, acc[c]);
+    }
+  }
+
+  const float unit = a.scale * __builtin_amdgcn_exp2f(-kWeightBits<T>);
+#pragma unroll
+  for (int c = 0; c < NB; ++c)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[c][i] = scaled.undo(acc[c][i]) * unit;
+  if constexpr (Shape::WK > 1) {
+    __syncthreads();
+    float* mine_at = reinterpret_cast<float*>(lds) + wave * 32 * DP;
+#pragma unroll
+    for (int c = 0; c < NB; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mine_at[(32 * c + result_row(i)) * 32 + lane % 32] = acc[c][i];
+    __syncthreads();
+    if (wk > 0) return;
+    for (int other = 1; other < Shape::WK; ++other) {
+      const float* at = reinterpret_cast<const float*>(lds) + (other * WR + wr) * 32 * DP;
+#pragma unroll
+      for (int c = 0; c < NB; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[c][i] += at[(32 * c + result_row(i)) * 32 + lane % 32];
+    }
+  }
+  if (!live) return;
+  // A split's sums lie in grad_q's own order.
+  const int64_t elements = int64_t(a.B) * a.Q * a.K * a.G * a.D;
+#pragma unroll
+  for (int c = 0; c < NB; ++c)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * c + 8 * g + 4 * (lane / 32);
+      const float v[4] = {acc[c][4 * g], acc[c][4 * g + 1], acc[c][4 * g + 2], acc[c][4 * g + 3]};
+      if (a.splits > 1)
+        store_four(a.part + split * elements + out_at + d, v, a.D - d, a.D % 4 == 0);
+      else
+        store_four(static_cast<T*>(a.grad_q) + out_at + d, v, a.D - d, a.out_vector);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Backward, states: a workgroup's 4 waves hold 32 keys each and walk over the rows (all of the
+// group's heads), so that dk and dv of a key are summed by one wave. Row splits leave fp32
+// sums, which sum_kernel adds in their order.
+
+template <typename T, int DP> struct StatesShape {
+  static constexpr int kKeys = 32 * kWaves;
+  static constexpr int RB = DP * int(sizeof(T)) <= 192 ? 2 : 1;  // blocks of 32 rows in a tile
+  static constexpr int kRows = 32 * RB;
+  static constexpr int kTile = kRows * Tile<T, DP>::kRowBytes;
+  static constexpr int kBuffers = 2;
+  static constexpr int kRowData = kRows * (3 * 4 + 8);
+  static constexpr int kLds = kBuffers * (2 * kTile + kRowData);
+};
+
+template <typename T, int DP, int MASK>
+__global__ __launch_bounds__(kThreads) void attention_grad_states_kernel(const Args a) {
+  using Shape = StatesShape<T, DP>;
+  using TileT = Tile<T, DP>;
+  constexpr int NB = DP / 32, kSteps = TileT::kPieces / 2, kRows = Shape::kRows;
+  constexpr int N = 16 / int(sizeof(T));
+  __shared__ __attribute__((aligned(16))) char lds[Shape::kLds];
+
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const uint32_t key_tiles = (uint32_t(a.S) + Shape::kKeys - 1) / Shape::kKeys;
+  uint32_t id = xcd_order(blockIdx.x, gridDim.x);
+  const int key_tile = int(id % key_tiles);
+  id /= key_tiles;
+  const int split = int(id % uint32_t(a.row_splits));
+  const int bk = int(id / uint32_t(a.row_splits));
+  const int b = bk / a.K, kv = bk % a.K;
+
+  const int states = states_of(a, b);
+  const int key = key_tile * Shape::kKeys + 32 * wave + lane % 32;
+  bool on = key < states;
+  if constexpr (MASK == kBoolMask)
+    if (a.mask_of_keys && on) on = bool_mask(a, b * a.mask_batch + int64_t(key) * a.mask_key);
+
+  u32x4 k[kSteps], v[kSteps];
+  {
+    const T* k_row = static_cast<const T*>(a.k) + b * a.k_batch + int64_t(key) * a.k_row + kv * a.k_head;
+    const T* v_row = static_cast<const T*>(a.v) + b * a.v_batch + int64_t(key) * a.v_row + kv * a.v_head;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int c = (2 * s + lane / 32) * N;
+      const u32x4 zero = {0, 0, 0, 0};
+      k[s] = on ? load_piece(k_row, c, a.D, a.vector) : zero;
+      v[s] = on ? load_piece(v_row, c, a.D, a.vector) : zero;
+    }
+  }
+
+  const int tiles = int((a.R + kRows - 1) / kRows);
+  int first = int(int64_t(tiles) * split / a.row_splits), last = int(int64_t(tiles) * (split + 1) / a.row_splits);
+  if (key_tile * Shape::kKeys >= states) last = first;  // padding only: zeros
+  const T* q_base = static_cast<const T*>(a.q) + b * a.q_batch;
+  const T* go_base = static_cast<const T*>(a.grad_out) + int64_t(b) * a.Q * a.K * a.G * a.D;
+  Stage<T, DP, kRows, kThreads> q_stage, go_stage;
+  float2 stat = {INFINITY, 0.0f};
+  float delta = 0.0f;
+  int64_t mask_at = 0;
+  auto load = [&](int tile) {
+    q_stage.load([&](int row) -> const T* {
+      const uint32_t r = uint32_t(tile) * kRows + row;
+      if (r >= a.R) return nullptr;
+      const RowOf o = row_of(a, kv, r);
+      return q_base + int64_t(o.query) * a.q_row + o.head * a.q_head;
+    }, a.D, a.vector);
+    go_stage.load([&](int row) -> const T* {
+      const uint32_t r = uint32_t(tile) * kRows + row;
+      if (r >= a.R) return nullptr;
+      const RowOf o = row_of(a, kv, r);
+      return go_base + (int64_t(o.query) * (a.K * a.G) + o.head) * a.D;
+    }, a.D, a.out_vector);
+    if (threadIdx.x < kRows) {
+      const uint32_t r = uint32_t(tile) * kRows + threadIdx.x;
+      const bool live = r < a.R;
+      stat = live ? a.row_stats[int64_t(bk) * a.R + r] : float2{INFINITY, 0.0f};
+      delta = live ? a.delta[int64_t(bk) * a.R + r] : 0.0f;
+      if constexpr (MASK != kNoMask) mask_at = mask_row_at(a, b, row_of(a, kv, live ? r : a.R - 1));
+    }
+  };
+
+  f32x16 grad_k[NB] = {}, grad_v[NB] = {};
+  Scaled<T> scaled;
+  const float factor = MASK == kFloatMask ? a.scale : a.scale * kLog2e;
+  if (first < last) load(first);
+  for (int tile = first; tile < last; ++tile) {
+    char* q_tile = lds + ((tile - first) % Shape::kBuffers) * (2 * Shape::kTile + Shape::kRowData);
+    char* go_tile = q_tile + Shape::kTile;
+    int64_t* row_mask = reinterpret_cast<int64_t*>(go_tile + Shape::kTile);
+    float* row_shift = reinterpret_cast<float*>(row_mask + kRows);
+    float* row_delta = row_shift + kRows;
+    float* row_max = row_delta + kRows;  // float masks only
+    q_stage.store(q_tile);
+    go_stage.store(go_tile);
+    if (threadIdx.x < kRows) {
+      row_shift[threadIdx.x] = kWeightBits<T> - (MASK == kFloatMask ? stat.y : stat.x + stat.y);
+      row_delta[threadIdx.x] = delta;
+      if constexpr (MASK == kFloatMask) row_max[threadIdx.x] = stat.x;
+      if constexpr (MASK != kNoMask) row_mask[threadIdx.x] = mask_at;
+    }
+    __syncthreads();
+    if (tile + 1 < last) load(tile + 1);
+
+#pragma unroll
+    for (int n = 0; n < Shape::RB; ++n) {
+      const int local = 32 * n;
+      float add[16];
+      uint32_t bits = on ? 0xffff : 0;
+      if constexpr (MASK == kBoolMask) {
+        if (on) {
+          bits = 0;
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            bits |= uint32_t(bool_mask(a, row_mask[local + result_row(i)] + int64_t(key) * a.mask_key)) << i;
+        }
+        if (!__any(bits != 0)) continue;
+      } else if constexpr (MASK == kFloatMask) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          add[i] = on ? float_mask(a, row_mask[local + result_row(i)] + int64_t(key) * a.mask_key) : kLowest;
+          if (add[i] == kLowest) bits &= ~(1u << i);
+        }
+      }
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int t = 0; t < kSteps; ++t) {
+        s = Mma<T>::rows(row_piece<T, DP>(q_tile, local, t), k[t], s);
+        dp = Mma<T>::rows(row_piece<T, DP>(go_tile, local, t), v[t], dp);
+      }
+      float p[16], ds[16];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int at = local + result_row(4 * g);
+        const f32x4 shift = *reinterpret_cast<const f32x4*>(row_shift + at);
+        const f32x4 dl = *reinterpret_cast<const f32x4*>(row_delta + at);
+        f32x4 top = {};
+        if constexpr (MASK == kFloatMask) top = *reinterpret_cast<const f32x4*>(row_max + at);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = 4 * g + j;
+          const float y = MASK == kFloatMask ? fmaf(fmaf(s[i], factor, add[i]) - top[j], kLog2e, shift[j])
+                                             : fmaf(s[i], factor, shift[j]);
+          const bool here = (bits >> i) & 1;
+          p[i] = here ? __builtin_amdgcn_exp2f(y) : 0.0f;
+          ds[i] = here ? p[i] * (dp[i] - dl[j]) : 0.0f;
+        }
+      }
+      const auto wp = Mma<T>::weights(p);
+#pragma unroll
+      for (int c = 0; c < NB; ++c) grad_v[c] = accumulate<T, DP>(go_tile, local, c, wp, grad_v[c]);
+      scaled.fit(ds, grad_k);
+      const auto ws = Mma<T>::weights(ds);
+#pragma unroll
+      for (int c = 0; c < NB; ++c) grad_k[c] = accumulate<T, DP>(q_tile, local, c, ws, grad_k[c]);
+    }
+  }
+
+  if (key >= a.S) return;
+  const float unit = __builtin_amdgcn_exp2f(-kWeightBits<T>);
+  const int64_t at = ((int64_t(b) * a.S + key) * a.K + kv) * a.D;
+  const int64_t elements = int64_t(a.B) * a.S * a.K * a.D;
+#pragma unroll
+  for (int c = 0; c < NB; ++c)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * c + 8 * g + 4 * (lane / 32);
+      float x[4], y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = scaled.undo(grad_k[c][4 * g + i]) * (unit * a.scale);
+        y[i] = grad_v[c][4 * g + i] * unit;
+      }
+      if (a.row_splits > 1) {
+        store_four(a.part_k + split * elements + at + d, x, a.D - d, a.D % 4 == 0);
+        store_four(a.part_v + split * elements + at + d, y, a.D - d, a.D % 4 == 0);
+      } else {
+        store_four(static_cast<T*>(a.grad_k) + at + d, x, a.D - d, a.out_vector);
+        store_four(static_cast<T*>(a.grad_v) + at + d, y, a.D - d, a.out_vector);
+      }
+    }
+}
+
+// out = the sum of `count` fp32 parts of n elements each, in their order.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_sum_kernel(const float* part, int count, int64_t n, T* out,
+                                                            const float* part2, T* out2) {
+  const int64_t at = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (at >= n) return;
+  if (blockIdx.y) {
+    part = part2;
+    out = out2;
+  }
+  float v[4] = {};
+  const bool vector = n % 4 == 0;
+  for (int s = 0; s < count; ++s) {
+    const float* p = part + s * n + at;
+    if (vector) {
+      const f32x4 four = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += four[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (at + i < n) v[i] += p[i];
+    }
+  }
+  store_four(out + at, v, int(n - at < 4 ? n - at : 4), vector && reinterpret_cast<uintptr_t>(out) % 16 == 0);
+}
+
+// ---------------------------------------------------------------------------
+// Launches, one translation unit for each type (attention_f32.hip and so on): the kernels'
+// variants compile side by side.
+
+template <int V> using Const = std::integral_constant<int, V>;
+
+template <typename F> void with_mask(int kind, F f) {
+  if (kind == kNoMask) f(Const<kNoMask>());
+  else if (kind == kBoolMask) f(Const<kBoolMask>());
+  else f(Const<kFloatMask>());
+}
+
+inline int padded(int64_t D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
+
+template <typename F> void with_channels(int64_t D, F f) {
+  switch (padded(D)) {
+    case 32: f(Const<32>()); break;
+    case 64: f(Const<64>()); break;
+    case 96: f(Const<96>()); break;
+    default: f(Const<128>()); break;
+  }
+}
+
+// `groups` and `key_groups`: workgroups of the walk over the keys and over the rows.
+template <typename T> void launch_forward(const Args& a, int mask_kind, bool few_rows, uint32_t groups, hipStream_t s);
+template <typename T>
+void launch_backward(const Args& a, int mask_kind, bool few_rows, uint32_t groups, uint32_t key_groups, hipStream_t s);
+
+#ifdef ATTENTION_DEFINE_LAUNCHES
+
+template <typename T> void launch_forward(const Args& a, int mask_kind, bool few_rows, uint32_t groups, hipStream_t s) {
+  with_channels(a.D, [&](auto dp) {
+    with_mask(mask_kind, [&](auto kind) {
+      constexpr int DP = decltype(dp)::value, MASK = decltype(kind)::value;
+      if constexpr (sizeof(T) * DP < 512)
+        if (few_rows) return attention_forward_kernel<T, DP, MASK, 1><<<groups, kThreads, 0, s>>>(a);
+      attention_forward_kernel<T, DP, MASK, 4><<<groups, kThreads, 0, s>>>(a);
+    });
+  });
+  if (a.splits > 1) {
+    const int64_t threads = int64_t(a.B) * a.K * a.R * ((a.D + 3) / 4);
+    attention_combine_kernel<T><<<uint32_t(ceil_div(threads, 256)), 256, 0, s>>>(a, mask_kind == kFloatMask);
+  }
+}
+
+template <typename T>
+void launch_backward(const Args& a, int mask_kind, bool few_rows, uint32_t groups, uint32_t key_groups, hipStream_t s) {
+  with_channels(a.D, [&](auto dp) {
+    with_mask(mask_kind, [&](auto kind) {
+      constexpr int DP = decltype(dp)::value, MASK = decltype(kind)::value;
+      bool done = groups == 0;
+      if constexpr (sizeof(T) * DP < 512)
+        if (few_rows && !done) {
+          attention_grad_q_kernel<T, DP, MASK, 1><<<groups, kThreads, 0, s>>>(a);
+          done = true;
+        }
+      if (!done) attention_grad_q_kernel<T, DP, MASK, 4><<<groups, kThreads, 0, s>>>(a);
+      if (key_groups) attention_grad_states_kernel<T, DP, MASK><<<key_groups, kThreads, 0, s>>>(a);
+    });
+  });
+  if (groups && a.splits > 1) {
+    const int64_t count = int64_t(a.B) * a.Q * a.K * a.G * a.D;
+    attention_sum_kernel<T><<<uint32_t(ceil_div(count, 1024)), 256, 0, s>>>(
+        a.part, a.splits, count, static_cast<T*>(a.grad_q), nullptr, nullptr);
+  }
+  if (key_groups && a.row_splits > 1) {
+    const int64_t count = int64_t(a.B) * a.S * a.K * a.D;
+    attention_sum_kernel<T><<<dim3(uint32_t(ceil_div(count, 1024)), 2), 256, 0, s>>>(
+        a.part_k, a.row_splits, count, static_cast<T*>(a.grad_k), a.part_v, static_cast<T*>(a.grad_v));
+  }
+}
+
+#define ATTENTION_INSTANTIATE(T)                                                                        \
+  namespace attention {                                                                                 \
+  template void launch_forward<T>(const Args&, int, bool, uint32_t, hipStream_t);                       \
+  template void launch_backward<T>(const Args&, int, bool, uint32_t, uint32_t, hipStream_t);            \
+  }
+
+#endif
+
+}  // namespace attention
+
+#endif  // DEFORMOPS_AMD_ATTENTION_H_

@@ -1,0 +1,5 @@
+// The cross attention kernels of one element type.
+#define ATTENTION_DEFINE_LAUNCHES
+#include "attention.h"
+
+ATTENTION_INSTANTIATE(float)

@@ -28,6 +28,7 @@
 #include <cstdlib>
 #include <string>
 
+#include "bridge.h"
 #include "deformops_amd.h"
 
 namespace {
@@ -251,4 +252,5 @@ PYBIND11_MODULE(_native, m) {
   m.def("init", &init);
   m.def("forward", &forward);
   m.def("try_forward", &try_forward);
+  define_operators(m);
 }

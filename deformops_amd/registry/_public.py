@@ -45,7 +45,7 @@ class _FoldVmap:
             if position in self.fixed:
                 if dim is not None:
                     raise RuntimeError(
-                        f"{self.fixed[position]} cannot be mapped by vmap: one pyramid describes every "
+                        f"{self.fixed[position]} cannot be mapped by vmap: one of it describes every "
                         f"image of the batch. Pass it with in_dims=None."
                     )
                 folded.append(arg)
@@ -70,15 +70,15 @@ class _FoldVmap:
 
 
 def define_public_op(name: str, schema: str, kernel: Callable[..., Any], *,
-                     fixed: Mapping[int, str] | None = None) -> Any:
+                     fixed: Mapping[int, str] | None = None, vmap: Callable[..., Any] | None = None) -> Any:
     """Define ``deformops::<name>`` with ``kernel`` as its composite implementation and
     the batch-folding vmap rule (``fixed``: positions vmap may not map, with their
-    names). A name that already exists is returned as it is."""
+    names), or the rule ``vmap``. A name that already exists is returned as it is."""
     namespace = getattr(torch.ops, NAMESPACE)
     if hasattr(namespace, name):
         return getattr(namespace, name)
     _LIBRARY.define(name + schema)
     _LIBRARY.impl(name, kernel, "CompositeImplicitAutograd")
     op = getattr(namespace, name)
-    torch.library.register_vmap(f"{NAMESPACE}::{name}", _FoldVmap(op, fixed or {}), lib=_LIBRARY)
+    torch.library.register_vmap(f"{NAMESPACE}::{name}", vmap or _FoldVmap(op, fixed or {}), lib=_LIBRARY)
     return op

@@ -283,6 +283,102 @@ int msda_record_plan(int value_dtype, int loc_dtype, int64_t batch, int64_t spat
                      int64_t points, int flags, int* chunk_queries, int* chunks,
                      int64_t* offsets);
 
+/* ---------------------------------------------------------------------------
+ * The operators beside MSDA. Pointers, streams and return codes are as above;
+ * deformops_last_error() holds the message of the calling thread's last failed call
+ * of a deformops_* function. MSDA_F64 is not taken. No counterpart in the reference.
+ */
+
+/*
+ * One cross attention call: softmax(scale * query key^T + mask) value for each image and
+ * head. Strides are in elements, for the axes named; the channels of a row lie side by
+ * side. The heads of a group of heads / key_heads share key head h / (heads / key_heads).
+ *
+ *   query       [batch, queries, heads, channels]     strides (batch, row, head)
+ *   key, value  [batch, keys, key_heads, channels]    strides (batch, row, head)
+ *   output      [batch, queries, heads * channels]    dense
+ *   mask        [batch, heads, queries, keys], stride 0 where it is one for an axis;
+ *               mask_kind 1: one byte each, non-zero where the row attends the key;
+ *               mask_kind 2: mask_dtype, added to the scaled scores (-inf removes the key)
+ *   key_lengths [batch] index_dtype, or null: keys at or past it are not read
+ *
+ * Keys that key_lengths or a mask of kind 1 with equal rows and heads (strides 0)
+ * removes may hold any value. A row that no key is left for gives zeros.
+ */
+typedef struct deformops_attention {
+  const void* query;
+  const void* key;
+  const void* value;
+  const void* mask;
+  const void* key_lengths;
+  void* output;
+  int64_t query_strides[3];
+  int64_t key_strides[3];
+  int64_t value_strides[3];
+  int64_t mask_strides[4];
+  int64_t batch, queries, keys, heads, key_heads, channels;
+  float scale;
+  int dtype;       /* of query, key, value, output and every gradient */
+  int mask_kind;   /* 0 none, 1 bytes, 2 additive */
+  int mask_dtype;
+  int index_dtype;
+} deformops_attention;
+
+/* Bytes of workspace the forward and the backward of such a call take (0: none); reads
+ * the sizes and types only. Host only. */
+int deformops_cross_attention_workspace_size(const deformops_attention* call, int64_t* forward,
+                                             int64_t* backward);
+
+/* Writes output and, unless row_stats is null, two floats for each (image, key head, query,
+ * head of the group), for the backward. The workspace is aligned to 256 bytes. */
+int deformops_cross_attention_forward(const deformops_attention* call, void* row_stats,
+                                      void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Writes the three gradients, dense in the layouts above, from the forward's output and
+ * row_stats and the dense grad_output. Sums are in fp32 and in an order that the sizes
+ * fix: equal calls give equal bits. The mask has no gradient. */
+int deformops_cross_attention_backward(const deformops_attention* call, const void* row_stats,
+                                       const void* grad_output, void* grad_query, void* grad_key,
+                                       void* grad_value, void* workspace, int64_t workspace_bytes,
+                                       void* stream);
+
+/* Element types of rotary positions. */
+enum deformops_position_type {
+  DEFORMOPS_POSITION_I64 = 0,
+  DEFORMOPS_POSITION_I32 = 1,
+  DEFORMOPS_POSITION_F32 = 2,
+  DEFORMOPS_POSITION_F64 = 3,
+};
+
+/*
+ * Rotary positions with several axes: y [batch, tokens, heads, channels], dense, is x (of
+ * strides batch, row, head in elements) with its pairs of channels turned by
+ * position[batch, token, axis of the pair] * frequencies[pair] (formed in 64 bits), or by
+ * minus that with `inverse`, which is the backward. Axis i rotates sections[i] pairs, in
+ * order; R pairs in all (at most 256), (j, j + R) or, `interleaved`, (2 j, 2 j + 1).
+ * Positions have strides (batch, token, axis), 0 where one serves all; frequencies are
+ * dense float32. y may not overlap x.
+ */
+int deformops_rotary(const void* x, const int64_t* x_strides, void* y, int dtype,
+                     const void* positions, const int64_t* position_strides, int position_type,
+                     const void* frequencies, const int64_t* sections, int64_t axes,
+                     int64_t batch, int64_t tokens, int64_t heads, int64_t channels,
+                     int interleaved, int inverse, void* stream);
+
+/*
+ * Dropout: y_i = x_i / (1 - p) where element i is kept and 0 where it is dropped, plus
+ * residual_i unless residual is null; dense tensors of one dtype. Element i is kept where
+ * word i % 4 of Philox4x32 with 7 rounds, counter (i / 4, offset), key seed, is at least
+ * round(p 2^32) (at most 2^32 - 1; p = 1 drops all). The seed is `seed`, or the int64 at
+ * seed_at in device memory when that is not null. The gradient of x is this call on the
+ * output's gradient without a residual. y may be x or residual.
+ */
+int deformops_dropout(const void* x, const void* residual, void* y, int dtype, int64_t elements,
+                      double p, uint64_t seed, const void* seed_at, uint64_t offset, void* stream);
+
+/* The message of the calling thread's last failed deformops_* call ("" if none). */
+const char* deformops_last_error(void);
+
 #ifdef __cplusplus
 }
 #endif

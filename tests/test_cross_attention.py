@@ -1,0 +1,601 @@
+"""Cross attention against its definition in 64 bits: outputs and gradients of both
+backends, masks that leave nothing, padding, layouts, refusals, tracing.
+
+Tolerances. With u half a step of the dtype (eps / 2), e = 2^-24, and s the scaled scores:
+
+- a score is off by at most e_s = e (D + 4) scale sum|q||k| + 4 e |s| + 2 e |mask| (its
+  sum, and the argument of the exponential), so a weight p is off by p (2 e_s + 4 e) (the
+  weight and its row's sum), and by u p where it becomes a 16-bit operand;
+- a sum of n terms in float32 adds n e times the sum of their magnitudes;
+- delta comes from the rounded output: off by u sum|do||o|;
+- ds is rounded once more (u |ds|), and every result once (u |result|);
+- below the normal numbers a rounding is off by half a smallest step instead of u: v_exp_f32
+  gives 0 below 2^-126, so a float32 weight is off by up to 2^-126 more; a float16 operand
+  holds weights times 2^14, whose smallest step 2^-24 is 2^-38 of a weight: off by 2^-39
+  more; and ds times a power of two that puts the largest of its row (in dq) or key (in dk)
+  above 2^11: off by 2^-25 / 2^11 = 2^-36 of that more.
+
+The bounds below add these up, element by element, in 64 bits.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+from torch import Tensor
+
+from deformops_amd.core.errors import NoBackendError
+from deformops_amd.registry import Backend, cross_attention
+
+F32, F16, BF16, F64 = torch.float32, torch.float16, torch.bfloat16, torch.float64
+E = 2.0**-24
+IDS = {F32: "f32", F16: "f16", BF16: "bf16", F64: "f64"}
+
+
+def full_mask(mask: Tensor | None, lengths: Tensor | None, B: int, H: int, Q: int, S: int):  # noqa: N803
+    """``(added, off)`` of shape ``(B, H, Q, S)`` in 64 bits, on the CPU."""
+    added, off = torch.zeros(B, H, Q, S, dtype=F64), torch.zeros(B, H, Q, S, dtype=torch.bool)
+    if mask is not None:
+        mask = mask.detach().cpu()
+        if mask.dtype == torch.bool:
+            off = off | ~mask
+        else:
+            off = off | (mask == -math.inf)
+            added = added + torch.where(mask == -math.inf, 0.0, mask.double())
+    if lengths is not None:
+        off = off | (torch.arange(S) >= lengths.cpu()[:, None, None, None])
+    return added, off
+
+
+def reference(q, k, v, mask=None, lengths=None, scale=None, grad=None):
+    """``{name: (value, bound)}`` in 64 bits; u in the bounds is that of ``q.dtype``."""
+    u = torch.finfo(q.dtype).eps / 2 if q.dtype != F64 else 0.0
+    weights_u = u if q.dtype in (F16, BF16) else 0.0
+    e = E if q.dtype != F64 else 2.0**-52
+    q_type = q.dtype
+    B, Q, H, D = q.shape
+    S, K = k.shape[1], k.shape[2]
+    G = H // K
+    scale = D**-0.5 if scale is None else scale
+    added, off = full_mask(mask, lengths, B, H, Q, S)
+    # What nobody reads may hold anything.
+    unread = off.all(2).all(1)[:, :, None, None]
+    q, k, v = q.detach().cpu().double(), k.detach().cpu().double(), v.detach().cpu().double()
+    k, v = torch.where(unread, 0.0, k), torch.where(unread, 0.0, v)
+    q4 = q.transpose(1, 2)
+    k4, v4 = (t.repeat_interleave(G, 2).transpose(1, 2) for t in (k, v))
+    s = q4 @ k4.transpose(2, 3) * scale
+    e_s = e * (D + 4) * scale * (q4.abs() @ k4.abs().transpose(2, 3)) + 4 * e * s.abs() + 2 * e * added.abs()
+    s = (s + added).masked_fill(off, -math.inf)
+    e_s = e_s.masked_fill(off, 0.0)
+    e_s = e_s + e_s.amax(-1, keepdim=True) if S else e_s
+    p = torch.softmax(s, -1).nan_to_num(nan=0.0) if S else s
+    attended = (~off).double()
+    w_err = p * (2 * e_s + (S + 8) * e) + 2.0**-126 * attended  # of a weight in float32
+    p_err = w_err + weights_u * p + (2.0**-39 * attended if q_type == F16 else 0.0)
+    o = p @ v4
+    o_err = p_err @ v4.abs() + S * e * (p @ v4.abs()) + u * o.abs()
+
+    def merged(t):  # (B, H, Q, D) -> (B, Q, H * D)
+        return t.transpose(1, 2).reshape(B, Q, H * D)
+
+    result = {"out": (merged(o), merged(o_err))}
+    if grad is None:
+        return result
+    go = grad.detach().cpu().double().view(B, Q, H, D).transpose(1, 2)
+
+    def grouped(t):  # (B, H, S, D) -> (B, S, K, D), the sum over a group's heads
+        return t.view(B, K, G, S, D).sum(2).transpose(1, 2)
+
+    dv = grouped(p.transpose(2, 3) @ go)
+    dv_err = grouped((p_err + Q * G * e * p).transpose(2, 3) @ go.abs()) + u * dv.abs()
+    dp, delta = go @ v4.transpose(2, 3), (go * o).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    o_here = o_err  # the saved output is the rounded one
+    delta_err = (go.abs() * (o_here + D * e * o.abs())).sum(-1, keepdim=True)
+    dp_err = D * e * (go.abs() @ v4.abs().transpose(2, 3))
+    ds_err = w_err * (dp - delta).abs() + p * (dp_err + delta_err) + (weights_u + 4 * e) * ds.abs()
+    step_q = step_k = 0.0
+    if q_type == F16 and S and Q:
+        step_q = 2.0**-36 * ds.abs().amax(3, keepdim=True) * attended
+        step_k = 2.0**-36 * ds.abs().amax(2, keepdim=True).view(B, K, G, 1, S).amax(2, keepdim=True)
+        step_k = step_k.expand(B, K, G, 1, S).reshape(B, H, 1, S) * attended
+    dq = scale * (ds @ k4)
+    dq_err = scale * ((ds_err + step_q + S * e * ds.abs()) @ k4.abs()) + u * dq.abs()
+    dk = scale * grouped(ds.transpose(2, 3) @ q4)
+    dk_err = scale * grouped((ds_err + step_k + Q * G * e * ds.abs()).transpose(2, 3) @ q4.abs()) + u * dk.abs()
+    result.update(q=(dq.transpose(1, 2), dq_err.transpose(1, 2)), k=(dk, dk_err), v=(dv, dv_err))
+    return result
+
+
+def assert_within(name: str, actual: Tensor, expected: tuple[Tensor, Tensor], tiny: float) -> None:
+    value, bound = expected
+    actual = actual.detach().cpu().double()
+    assert actual.shape == value.shape
+    assert actual.isfinite().all(), f"{name}: {int((~actual.isfinite()).sum())} values are not finite"
+    over = (actual - value).abs() - (1.001 * bound + tiny)  # the bounds hold to first order
+    if over.numel():
+        at = int(over.argmax())
+        assert over.max() <= 0, (f"{name}: {actual.flatten()[at]} is not {value.flatten()[at]} to "
+                                 f"{bound.flatten()[at]} (element {at})")
+
+
+def tiny_of(dtype: torch.dtype) -> float:
+    """Half the smallest step of the dtype, which bounds the rounding of values near zero."""
+    return torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2 + 1e-37
+
+
+def run_and_check(q, k, v, *, mask=None, lengths=None, scale=None, grad=None, backend=None) -> dict[str, Tensor]:
+    expected = reference(q, k, v, mask, lengths, scale, grad)
+    leaves = [t.detach().requires_grad_(grad is not None) for t in (q, k, v)]
+    out = cross_attention(*leaves, mask=mask, key_lengths=lengths, scale=scale, backend=backend)
+    assert out.dtype == q.dtype and out.is_contiguous()
+    got = {"out": out.detach()}
+    if grad is not None:
+        got.update(zip("qkv", torch.autograd.grad(out, leaves, grad)))
+        for name, t in zip("qkv", (q, k, v)):
+            assert got[name].dtype == t.dtype and got[name].shape == t.shape
+    for name, pair in expected.items():
+        assert_within(name, got[name], pair, tiny_of(q.dtype))
+    return got
+
+
+def tensors(B, Q, S, H, K, D, dtype, device, *, seed=0, spread=1.0):  # noqa: N803
+    g = torch.Generator().manual_seed(seed)
+    shapes = ((B, Q, H, D), (B, S, K, D), (B, S, K, D), (B, Q, H * D))
+    q, k, v, grad = (torch.randn(*s, generator=g, dtype=F64) for s in shapes)
+    return [t.to(dtype).to(device) for t in (q * spread, k, v, grad)]
+
+
+def make_mask(kind: str, B, H, Q, S, device, *, seed=1):  # noqa: N803
+    g = torch.Generator().manual_seed(seed)
+    if kind == "none":
+        return None
+    if kind == "bool":  # some rows empty, some tiles empty
+        mask = torch.rand(B, H, Q, S, generator=g) < 0.4
+        mask[..., S // 3: S // 3 + 70] = False
+        mask[:, :, ::5] = False
+    elif kind == "heads":  # one for all heads
+        mask = torch.rand(B, 1, Q, S, generator=g) < 0.5
+    elif kind == "rows":  # 2 axes
+        mask = torch.rand(Q, S, generator=g) < 0.5
+    elif kind == "states":  # padding
+        mask = torch.rand(B, 1, 1, S, generator=g) < 0.6
+    elif kind == "padded":  # rows of a wider tensor, aligned
+        mask = (torch.rand(B, 1, Q, (S + 3) // 4 * 4, generator=g) < 0.5)[..., :S]
+    elif kind == "turned":  # keys are not side by side
+        mask = (torch.rand(B, S, Q, 1, generator=g) < 0.5).permute(0, 3, 2, 1)
+    elif kind in ("float", "float16", "floatbf16"):
+        mask = 2 * torch.randn(B, H, Q, S, generator=g)
+        mask[torch.rand(B, H, Q, S, generator=g) < 0.2] = -math.inf
+        mask[:, :, ::7] = -math.inf
+        mask = mask.to({"float": F32, "float16": F16, "floatbf16": BF16}[kind])
+    elif kind == "lowest":  # finite, yet far below every score: such rows stay uniform
+        mask = torch.zeros(1, 1, Q, S)
+        mask[:, :, 1::2] = torch.finfo(F32).min
+        mask[:, :, ::2, : S // 2] = torch.finfo(F32).min
+    return mask.to(device)
+
+
+BACKENDS = [pytest.param("cpu", id="cpu"), pytest.param("cuda", id="gpu", marks=pytest.mark.gpu)]
+SIZES = [  # B, Q, S, H, K, D
+    (1, 1, 1, 1, 1, 1),
+    (2, 1, 300, 8, 2, 64),
+    (1, 3, 129, 4, 1, 32),
+    (2, 37, 65, 2, 2, 16),
+    (1, 130, 31, 3, 3, 40),
+    (2, 100, 257, 6, 2, 80),
+    (1, 64, 640, 2, 1, 128),
+    (3, 5, 33, 4, 4, 7),
+    (1, 33, 512, 2, 2, 96),
+    (1, 700, 77, 2, 2, 64),
+]
+
+
+def on(device: str) -> str:
+    if device == "cuda" and not torch.cuda.is_available():
+        pytest.skip("no ROCm GPU")
+    return device
+
+
+@pytest.mark.parametrize("device", BACKENDS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=IDS.get)
+@pytest.mark.parametrize("sizes", SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_outputs_and_gradients(device, sizes, dtype):
+    q, k, v, grad = tensors(*sizes, dtype, on(device))
+    run_and_check(q, k, v, grad=grad)
+
+
+@pytest.mark.parametrize("device", BACKENDS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=IDS.get)
+@pytest.mark.parametrize("kind", ["bool", "heads", "rows", "states", "padded", "turned", "float", "float16", "floatbf16",
+                                  "lowest"])
+@pytest.mark.parametrize("sizes", [(2, 45, 203, 4, 2, 32), (1, 1, 130, 2, 1, 48), (1, 150, 64, 1, 1, 64)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_masks(device, sizes, kind, dtype):
+    B, Q, S, H, _, _ = sizes
+    q, k, v, grad = tensors(*sizes, dtype, on(device))
+    got = run_and_check(q, k, v, mask=make_mask(kind, B, H, Q, S, device), grad=grad)
+    if kind in ("bool", "float") and Q > 1:  # rows that nothing is left for
+        step = 5 if kind == "bool" else 7
+        assert got["out"][:, ::step].eq(0).all() and got["q"][:, ::step].eq(0).all()
+
+
+@pytest.mark.parametrize("device", BACKENDS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=IDS.get)
+@pytest.mark.parametrize("index", [torch.int32, torch.int64], ids=["i32", "i64"])
+@pytest.mark.parametrize("queries", [1, 140])
+def test_lengths_leave_what_is_behind_them_unread(device, dtype, index, queries):
+    lengths = torch.tensor([0, 1, 64, 200, 1000, -3], dtype=index, device=on(device))
+    q, k, v, grad = tensors(6, queries, 200, 4, 2, 64, dtype, device)
+    for b, n in enumerate([0, 1, 64, 200, 200, 0]):
+        k[b, n:], v[b, n:] = math.nan, math.inf
+    got = run_and_check(q, k, v, lengths=lengths.clamp(0, 200), grad=grad)
+    again = run_and_check(q, k, v, lengths=lengths, grad=grad)
+    for name in got:
+        assert torch.equal(got[name], again[name])
+    assert got["out"][0].eq(0).all() and got["k"][1, 1:].eq(0).all() and got["v"][2, 64:].eq(0).all()
+
+
+@pytest.mark.parametrize("device", BACKENDS)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=IDS.get)
+def test_a_mask_of_states_leaves_them_unread(device, dtype):
+    q, k, v, grad = tensors(2, 40, 150, 4, 2, 32, dtype, on(device))
+    mask = make_mask("states", 2, 4, 40, 150, device)
+    mask[1] = False
+    gone = ~mask[:, 0, 0]
+    k[gone], v[gone] = math.nan, -math.inf
+    got = run_and_check(q, k, v, mask=mask, grad=grad)
+    assert got["k"][gone].eq(0).all() and got["v"][gone].eq(0).all() and got["out"][1].eq(0).all()
+    # and together with lengths
+    run_and_check(q, k, v, mask=mask, lengths=torch.tensor([99, 0], device=device), grad=grad)
+
+
+@pytest.mark.parametrize("device", BACKENDS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=IDS.get)
+def test_layouts(device, dtype):
+    """Heads first, a packed projection, a batch that is one tensor for all, odd offsets."""
+    q, k, v, grad = tensors(2, 50, 90, 4, 4, 24, dtype, on(device))
+    expected = run_and_check(q, k, v, grad=grad)
+    heads_first = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)]
+    packed = torch.cat([k, v], -1)
+    odd = torch.empty(k.numel() + 1, dtype=dtype, device=device)[1:].view(k.shape).copy_(k)
+    channels = torch.empty(2, 4, 24, 90, dtype=dtype, device=device).copy_(v.permute(0, 2, 3, 1)).permute(0, 3, 1, 2)
+    for layout in (heads_first, (q, packed[..., :24], packed[..., 24:]), (q, odd, v), (q, k, channels)):
+        got = run_and_check(*layout, grad=grad)
+        for name in got:
+            torch.testing.assert_close(got[name], expected[name], rtol=0, atol=0)
+    one = k[:1].expand(2, -1, -1, -1)
+    got = run_and_check(q, one, v, grad=grad)
+    for b in range(2):
+        alone = run_and_check(q[b:b + 1], k[:1], v[b:b + 1], grad=grad[b:b + 1])
+        torch.testing.assert_close(got["out"][b], alone["out"][0], rtol=2e-2, atol=2e-2)
+
+
+@pytest.mark.parametrize("device", BACKENDS)
+@pytest.mark.parametrize("sizes", [(0, 3, 4, 2, 2, 8), (2, 0, 4, 2, 1, 8), (2, 3, 0, 2, 1, 8), (1, 0, 0, 1, 1, 8)],
+                         ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("masked", [False, True])
+def test_empty_calls(device, sizes, masked):
+    B, Q, S, H, K, D = sizes
+    q, k, v, grad = tensors(*sizes, F32, on(device))
+    mask = torch.ones(B, H, Q, S, dtype=torch.bool, device=device) if masked else None
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = cross_attention(*leaves, mask=mask)
+    assert out.shape == (B, Q, H * D) and out.eq(0).all()
+    for leaf, g in zip(leaves, torch.autograd.grad(out, leaves, grad, allow_unused=True)):
+        assert g is None or (g.shape == leaf.shape and g.eq(0).all())
+
+
+@pytest.mark.parametrize("device", BACKENDS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=IDS.get)
+def test_scale_and_peaked_scores(device, dtype):
+    """Scores of hundreds: the running maximum moves, most weights vanish."""
+    q, k, v, grad = tensors(1, 70, 400, 2, 2, 64, dtype, on(device), spread=12.0)
+    k = k * torch.linspace(0.1, 3.0, 400, device=device).view(1, -1, 1, 1).to(dtype)
+    run_and_check(q, k, v, grad=grad)
+    run_and_check(q, k, v, grad=grad, scale=0.01)
+    run_and_check(q, k, v, grad=grad, scale=1.5)
+
+
+@pytest.mark.parametrize("device", BACKENDS)
+@pytest.mark.parametrize("size", [1e-4, 30.0])
+def test_half_gradients_keep_their_precision_at_any_size(device, size):
+    """Weights near 1 / 3000 times gradients of 1e-4 are far below float16's normal range,
+    and the sums they make are not. The incoming gradients differ by row, too."""
+    q, k, v, grad = tensors(1, 64, 3001, 2, 2, 32, F16, on(device), spread=0.3)
+    grad = (grad.float() * size * torch.logspace(-2, 0, 64, device=device).view(1, -1, 1)).to(F16)
+    got = run_and_check(q, k, v, grad=grad)
+    expected = reference(q, k, v, grad=grad)
+    for name in "kv":
+        value = expected[name][0]
+        error = (got[name].cpu().double() - value).norm() / value.norm()
+        assert error < 2 * torch.finfo(F16).eps + 2.0**-25 * value.numel() ** 0.5 / value.norm()
+
+
+@pytest.mark.parametrize("device", BACKENDS)
+def test_nan_and_infinity_reach_what_reads_them(device):
+    q, k, v, _ = tensors(1, 40, 70, 2, 2, 32, F32, on(device))
+    q[0, 3, 1, 5] = math.nan
+    out = cross_attention(q, k, v).view(1, 40, 2, 32)
+    assert out[0, 3, 1].isnan().all()
+    out[0, 3, 1] = 0
+    assert out.isfinite().all()
+    v[0, 69, 0, 2] = math.inf
+    out = cross_attention(q, k, v).view(1, 40, 2, 32)
+    assert out[0, :, 0, 2].eq(math.inf).all()
+
+
+@pytest.mark.parametrize("device", BACKENDS)
+def test_gradients_by_differences(device):
+    """Directional derivatives in 64 bits on the CPU, in float32 (steps of 2^-7) on the GPU."""
+    dtype = F64 if device == "cpu" else F32
+    step, tolerance = (1e-5, 1e-8) if device == "cpu" else (2.0**-7, 2e-3)
+    q, k, v, grad = tensors(2, 9, 41, 4, 2, 16, dtype, on(device))
+    mask = make_mask("bool", 2, 4, 9, 41, device)
+    lengths = torch.tensor([41, 17], device=device)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+
+    def value(*at):
+        return float((cross_attention(*at, mask=mask, key_lengths=lengths).double() * grad.double()).sum())
+
+    grads = torch.autograd.grad(cross_attention(*leaves, mask=mask, key_lengths=lengths), leaves, grad)
+    for i, g in enumerate(grads):
+        way = torch.randn(g.shape, generator=torch.Generator().manual_seed(i), dtype=F64).to(device, dtype)
+        with torch.no_grad():
+            ahead = [t + step * way if i == j else t for j, t in enumerate(leaves)]
+            back = [t - step * way if i == j else t for j, t in enumerate(leaves)]
+            slope = (value(*ahead) - value(*back)) / (2 * step)
+        wanted = float((g.double() * way.double()).sum())
+        assert abs(slope - wanted) <= tolerance * max(1.0, float(g.double().norm() * way.double().norm()) ** 0.5)
+
+
+# Refusals, on metadata alone.
+
+
+def bad(**changes):
+    q, k, v, _ = tensors(2, 3, 5, 4, 2, 8, F32, "cpu")
+    call = {"q": q, "k": k, "v": v, "mask": None, "lengths": None, "scale": None}
+    call.update(changes)
+    return call
+
+
+REFUSALS = {
+    "rank": (bad(q=torch.zeros(2, 3, 32)), ValueError, "query"),
+    "batch": (bad(k=torch.zeros(1, 5, 2, 8), v=torch.zeros(1, 5, 2, 8)), ValueError, "key has batch"),
+    "channels": (bad(k=torch.zeros(2, 5, 2, 4), v=torch.zeros(2, 5, 2, 4)), ValueError, "channels"),
+    "value": (bad(v=torch.zeros(2, 6, 2, 8)), ValueError, "value"),
+    "heads": (bad(k=torch.zeros(2, 5, 3, 8), v=torch.zeros(2, 5, 3, 8)), ValueError, "multiple"),
+    "no heads": (bad(q=torch.zeros(2, 3, 0, 8)), ValueError, "heads"),
+    "dtype": (bad(k=torch.zeros(2, 5, 2, 8, dtype=F16)), ValueError, "dtype"),
+    "integers": (bad(q=torch.zeros(2, 3, 4, 8, dtype=torch.int32)), ValueError, "floating"),
+    "mask rank": (bad(mask=torch.ones(2, 3, 5, dtype=torch.bool)), ValueError, "mask"),
+    "mask size": (bad(mask=torch.ones(3, 6, dtype=torch.bool)), ValueError, "mask"),
+    "mask dtype": (bad(mask=torch.ones(3, 5, dtype=torch.int32)), ValueError, "mask"),
+    "mask gradient": (bad(mask=torch.zeros(3, 5, requires_grad=True)), NotImplementedError, "mask"),
+    "lengths dtype": (bad(lengths=torch.zeros(2)), ValueError, "key_lengths"),
+    "lengths size": (bad(lengths=torch.zeros(3, dtype=torch.int64)), ValueError, "key_lengths"),
+    "scale": (bad(scale=0.0), ValueError, "scale"),
+    "scale sign": (bad(scale=-1.0), ValueError, "scale"),
+    "scale size": (bad(scale=1e-60), ValueError, "scale"),
+    "scale nan": (bad(scale=math.nan), ValueError, "scale"),
+    "device": (bad(lengths=torch.zeros(2, dtype=torch.int64, device="meta")), ValueError, "device"),
+}
+
+
+@pytest.mark.parametrize("device", BACKENDS)
+@pytest.mark.parametrize("name", REFUSALS)
+def test_refusals(device, name):
+    call, error, words = REFUSALS[name]
+    on(device)
+
+    def moved(t):
+        if not isinstance(t, Tensor) or t.device.type == "meta":
+            return t
+        return t.detach().to(device).requires_grad_(t.requires_grad)
+
+    with pytest.raises(error, match=words):
+        cross_attention(*(moved(call[n]) for n in "qkv"), mask=moved(call["mask"]),
+                        key_lengths=moved(call["lengths"]), scale=call["scale"])
+
+
+def test_call_surface():
+    q, k, v, _ = tensors(1, 2, 3, 1, 1, 8, F32, "cpu")
+    with pytest.raises(TypeError, match="positionally"):
+        cross_attention(q, k)
+    with pytest.raises(TypeError, match="unexpected"):
+        cross_attention(q, k, v, dropout=0.1)
+    with pytest.raises(TypeError, match="Backend"):
+        cross_attention(q, k, v, backend="eager")
+    assert cross_attention.resolve(q, k, v).backend is Backend.EAGER
+    torch.testing.assert_close(cross_attention(q, k, v, backend=Backend.EAGER), cross_attention(q, k, v))
+
+
+@pytest.mark.gpu
+def test_gpu_calls_that_no_kernel_takes(device):
+    for sizes, dtype in (((1, 2, 3, 1, 1, 8), F64), ((1, 2, 3, 1, 1, 129), F32)):
+        q, k, v, _ = tensors(*sizes, dtype, device)
+        with pytest.raises(NoBackendError):
+            cross_attention(q, k, v)
+    with pytest.raises(NoBackendError):
+        cross_attention(*(t.cpu() for t in (q, k, v)), backend=Backend.HIP)
+
+
+@pytest.mark.parametrize("device", BACKENDS)
+def test_vmap_and_the_public_operator(device):
+    q, k, v, _ = tensors(6, 4, 21, 4, 2, 16, F32, on(device))
+    mask = make_mask("heads", 6, 4, 4, 21, device)
+    lengths = torch.tensor([21, 3, 0, 21, 7, 20], device=device)
+    whole = cross_attention(q, k, v, mask=mask, key_lengths=lengths)
+
+    def split(t):
+        return t.view(3, 2, *t.shape[1:])
+
+    mapped = torch.vmap(lambda *t: cross_attention(t[0], t[1], t[2], mask=t[3], key_lengths=t[4]))(
+        split(q), split(k), split(v), split(mask), split(lengths))
+    torch.testing.assert_close(mapped.reshape(whole.shape), whole, rtol=1e-6, atol=1e-6)
+    shared = torch.vmap(lambda a: cross_attention(a, k[:2], v[:2], mask=mask[0, 0]))(split(q))
+    torch.testing.assert_close(shared[1], cross_attention(q[2:4], k[:2], v[:2], mask=mask[0, 0]), rtol=1e-6, atol=1e-6)
+    public = torch.ops.deformops.cross_attention(q, k, v, mask, lengths, 0.25)
+    torch.testing.assert_close(public, cross_attention(q, k, v, mask=mask, key_lengths=lengths, scale=0.25))
+
+
+@pytest.mark.parametrize("device", BACKENDS)
+def test_traced_calls_and_their_gradients(device):
+    q, k, v, grad = tensors(2, 5, 33, 4, 2, 32, F32, on(device))
+    lengths = torch.tensor([33, 9], device=device)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    expected = cross_attention(*leaves, key_lengths=lengths)
+    grads = torch.autograd.grad(expected, leaves, grad)
+
+    def call(*t):
+        return cross_attention(*t, key_lengths=lengths)
+
+    compiled = torch.compile(call, backend="aot_eager", fullgraph=True)(*leaves)
+    torch.testing.assert_close(compiled, expected, rtol=1e-6, atol=1e-6)
+    for got, wanted in zip(torch.autograd.grad(compiled, leaves, grad), grads):
+        torch.testing.assert_close(got, wanted, rtol=1e-5, atol=1e-6)
+    with torch._subclasses.fake_tensor.FakeTensorMode() as mode:
+        fake = [mode.from_tensor(t) for t in (*leaves, lengths)]
+        assert cross_attention(*fake[:3], key_lengths=fake[3]).shape == expected.shape
+
+
+@pytest.mark.parametrize("device", BACKENDS)
+def test_second_derivatives_and_tangents(device):
+    q, k, v, _ = tensors(1, 3, 5, 1, 1, 8, F32, on(device))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    if device == "cuda":
+        first = torch.autograd.grad(cross_attention(*leaves).pow(2).sum(), leaves[0], create_graph=True)[0]
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            first.sum().backward()
+        import torch.autograd.forward_ad as fwad  # noqa: PLC0415
+
+        with fwad.dual_level(), pytest.raises(NotImplementedError):
+            cross_attention(fwad.make_dual(q.detach(), torch.ones_like(q)), k, v)
+    else:
+        torch.autograd.grad(cross_attention(*leaves).pow(2).sum(), leaves[0], create_graph=True)
+
+
+# GPU: streams, graphs, long axes.
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=IDS.get)
+def test_equal_calls_give_equal_bits(device, dtype):
+    q, k, v, grad = tensors(1, 300, 900, 4, 2, 64, dtype, device)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    runs = []
+    for _ in range(3):
+        out = cross_attention(*leaves)
+        runs.append((out.detach(), *torch.autograd.grad(out, leaves, grad)))
+    for other in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+
+
+@pytest.mark.gpu
+def test_another_stream_and_two_at_once(device):
+    calls = [tensors(2, 120, 700, 4, 4, 64, BF16, device, seed=s) for s in range(2)]
+    expected = [run_and_check(*c[:3], grad=c[3]) for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    got = []
+    for stream, (q, k, v, grad) in zip(streams, calls):
+        with torch.cuda.stream(stream):
+            leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+            out = cross_attention(*leaves)
+            got.append((out.detach(), *torch.autograd.grad(out, leaves, grad)))
+    torch.cuda.synchronize()
+    for e, g in zip(expected, got):
+        assert all(torch.equal(a, b) for a, b in zip(e.values(), g))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("queries", [1, 200])
+def test_calls_replay_from_graphs(device, queries):
+    """Two captured graphs, forward and backward, replayed in turn with eager work between."""
+    sizes = (2, queries, 1500, 4, 2, 64)
+    inputs = [tensors(*sizes, BF16, device, seed=s) for s in range(4)]
+    lengths = torch.tensor([1500, 333], device=device)
+
+    def call(q, k, v, grad):
+        out = cross_attention(q, k, v, key_lengths=lengths)
+        return (out.detach(), *torch.autograd.grad(out, (q, k, v), grad))
+
+    statics, graphs, outs = [], [], []
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for n in range(2):
+            static = [t.clone() for t in inputs[n]]
+            for t in static[:3]:
+                t.requires_grad_()
+            call(*static)  # warm
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                outs.append(call(*static))
+            statics.append(static)
+            graphs.append(graph)
+    torch.cuda.synchronize()
+    for turn in range(3):
+        for n in range(2):
+            fresh = inputs[(turn + n) % 4]
+            with torch.no_grad():
+                for to, t in zip(statics[n], fresh):
+                    to.copy_(t)
+            graphs[n].replay()
+        torch.cuda.synchronize()
+        for n in range(2):
+            fresh = inputs[(turn + n) % 4]
+            leaves = [t.detach().requires_grad_() for t in fresh[:3]]
+            for a, b in zip(outs[n], call(*leaves, fresh[3])):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("queries", [1, 40])
+def test_a_cache_whose_offsets_pass_32_bits(device, queries):
+    """The second image's states lie past 2^31 elements."""
+    S, K, D = 131072, 64, 160 - 32  # noqa: N806
+    k = torch.zeros(2, S + 1024, K, D, dtype=BF16, device=device)
+    assert k[1, 1024:].storage_offset() > 2**30 and k.numel() > 2**31 - 1
+    g = torch.Generator(device).manual_seed(3)
+    rows = torch.randn(1, 512, K, D, generator=g, device=device).to(BF16)
+    k[1, S - 512 + 1024:] = rows[0]
+    q = torch.randn(2, queries, K, D, generator=g, device=device).to(BF16)
+    mask = torch.zeros(1, 1, 1, S + 1024, dtype=torch.bool, device=device)
+    mask[..., S + 512:] = True
+    out = cross_attention(q, k, k, mask=mask)
+    expected = reference(q[1:], rows, rows)["out"]
+    assert_within("out", out[1:], expected, tiny_of(BF16))
+    assert out[0].eq(0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
+@pytest.mark.parametrize("sizes", [(1, 1, 70001, 8, 1, 64), (2, 9, 9001, 4, 4, 32), (1, 5003, 45, 2, 1, 128)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_long_axes_are_split_and_joined(device, sizes, dtype):
+    B, Q, S, H, K, D = sizes
+    q, k, v, grad = tensors(*sizes, dtype, device)
+    lengths = torch.tensor([S - 17] + [S // 3] * (B - 1), device=device)
+    run_and_check(q, k, v, lengths=lengths, grad=grad)
+    run_and_check(q, k, v, mask=make_mask("states", B, H, Q, S, device), grad=grad)
+
+
+@pytest.mark.gpu
+def test_a_captured_backward_next_to_a_live_graph_of_its_leaves_is_refused(device):
+    q, k, v, grad = tensors(1, 20, 40, 2, 2, 32, BF16, device)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    alive = cross_attention(*leaves)  # holds the leaves' accumulators on the current stream
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), pytest.raises(RuntimeError, match="still lives"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+            torch.autograd.grad(cross_attention(*leaves), leaves, grad)
+    torch.cuda.synchronize()
+    expected = torch.autograd.grad(alive, leaves, grad)
+    del alive
+    for a, b in zip(torch.autograd.grad(cross_attention(*leaves), leaves, grad), expected):
+        assert torch.equal(a, b)
