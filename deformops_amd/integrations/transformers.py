@@ -4,7 +4,9 @@ Restates the reference ``integrations/transformers.py:1-282``: a drop-in for
 Deformable DETR's parameter-free attention core, one for Mask2Former's pixel
 decoder attention (which keeps the pretrained projections of the module it
 replaces), and :func:`patch`, which swaps both kinds in a model. The sampling runs
-on the HIP kernels through :func:`~deformops_amd.integrations._ops.run_msda`.
+on the HIP kernels through :func:`~deformops_amd.integrations._ops.run_msda`. On
+request ``patch`` also replaces the masked attention of Mask2Former's decoder, which
+the reference leaves alone, by cross attention on the HIP kernels.
 """
 
 from __future__ import annotations
@@ -15,6 +17,8 @@ from typing import TYPE_CHECKING
 import torch
 from torch import Tensor, nn
 
+from ..registry import Backend as RegistryBackend
+from ..registry import cross_attention
 from ._ops import run_msda
 from ._patch import patch_modules
 
@@ -42,6 +46,7 @@ except (ImportError, AttributeError) as exc:  # pragma: no cover
     raise ImportError(msg) from exc
 
 __all__ = [
+    "Mask2FormerMaskedCrossAttention",
     "Mask2FormerPixelDecoderEncoderMultiscaleDeformableAttention",
     "MultiScaleDeformableAttention",
     "patch",
@@ -182,11 +187,83 @@ class Mask2FormerPixelDecoderEncoderMultiscaleDeformableAttention(_UpstreamM2F):
         return self.output_proj(output), weights.view(B, Q, H, L, P)
 
 
+class Mask2FormerMaskedCrossAttention(nn.Module):
+    """Mask2Former's masked attention of its decoder's queries over one level of the pixel
+    decoder, on :data:`~deformops_amd.registry.cross_attention`.
+
+    Built from the ``nn.MultiheadAttention`` it replaces: the parameters are that module's
+    own, under their names, so pretrained weights, checkpoints and optimizer state carry
+    over. The attention weights are not formed: ``None`` stands in their place. The
+    reference leaves this module as it is.
+    """
+
+    def __init__(self, other: nn.MultiheadAttention, *, backend: Backend | None = None) -> None:
+        super().__init__()
+        if other.in_proj_weight is None or other.bias_k is not None or other.add_zero_attn or other.batch_first:
+            msg = "only a MultiheadAttention of one width, sequence first and without extra keys is replaced"
+            raise ValueError(msg)
+        if other.dropout:
+            msg = (
+                f"the attention module drops attention weights (p = {other.dropout}), which the "
+                f"cross attention kernels do not; patch the model with decoder=False"
+            )
+            raise ValueError(msg)
+        self.embed_dim = other.embed_dim
+        self.num_heads = other.num_heads
+        self.in_proj_weight = other.in_proj_weight
+        self.register_parameter("in_proj_bias", other.in_proj_bias)
+        self.out_proj = other.out_proj
+        self.backend = backend
+        self.training = other.training
+
+    def forward(
+        self,
+        query: Tensor,
+        key: Tensor,
+        value: Tensor,
+        key_padding_mask: Tensor | None = None,
+        attn_mask: Tensor | None = None,
+    ) -> tuple[Tensor, None]:
+        """``nn.MultiheadAttention``'s contract: inputs ``(length, batch, width)``, boolean
+        masks ``True`` where a state is left out, ``attn_mask`` ``(Q, S)`` or ``(batch *
+        heads, Q, S)``, boolean or added to the scores."""
+        Q, B, E = query.shape
+        S, H = key.shape[0], self.num_heads
+        biases = (None,) * 3 if self.in_proj_bias is None else self.in_proj_bias.chunk(3)
+
+        def heads(x: Tensor, weight: Tensor, bias: Tensor | None) -> Tensor:  # (B, length, H, D)
+            return nn.functional.linear(x, weight, bias).view(x.shape[0], B, H, E // H).transpose(0, 1)
+
+        q, k, v = (heads(x, w, b) for x, w, b in zip((query, key, value), self.in_proj_weight.chunk(3), biases))
+        mask = None
+        if attn_mask is not None:
+            mask = attn_mask if attn_mask.dim() == 2 else attn_mask.view(B, H, Q, S)  # noqa: PLR2004
+            if mask.dtype == torch.bool:
+                mask = ~mask
+        if key_padding_mask is not None:
+            kept = ~key_padding_mask.view(B, 1, 1, S)
+            if mask is None:
+                mask = kept
+            elif mask.dtype == torch.bool:
+                mask = mask.expand(B, H, Q, S) & kept
+            else:
+                mask = mask.expand(B, H, Q, S).masked_fill(~kept, -torch.inf)
+        out = cross_attention(q, k, v, mask=mask, backend=self.backend)
+        return self.out_proj(out.transpose(0, 1)), None
+
+
+def _with_cross_attention(layer: nn.Module, backend: Backend | None) -> nn.Module:
+    if isinstance(layer.cross_attn, nn.MultiheadAttention):
+        layer.cross_attn = Mask2FormerMaskedCrossAttention(layer.cross_attn, backend=backend)
+    return layer
+
+
 def patch(
     model: nn.Module,
     *,
     backend: Backend | MSDABackend | None = None,
     strict: bool = True,
+    decoder: bool = False,
 ) -> nn.Module:
     """Replace the model's Hugging Face MSDA modules of both kinds, in place.
 
@@ -200,6 +277,11 @@ def patch(
     strict
         Raise when nothing matched (the installed ``transformers`` may name the
         modules differently).
+    decoder
+        Also replace the masked attention of Mask2Former's decoder layers by
+        :class:`Mask2FormerMaskedCrossAttention`. Off by default: the replaced modules
+        return no attention weights. ``backend`` has to be a ``Backend`` member or
+        ``None`` then.
 
     Returns
     -------
@@ -210,9 +292,16 @@ def patch(
     RuntimeError
         If ``strict`` and no module was replaced.
     """
+    layers = []
+    if decoder:
+        if backend is not None and not isinstance(backend, RegistryBackend):
+            msg = f"decoder=True takes a Backend member or None, not {type(backend).__name__}"
+            raise TypeError(msg)
+        layers = [(_m2f.Mask2FormerMaskedAttentionDecoderLayer, lambda old: _with_cross_attention(old, backend))]
     return patch_modules(
         model,
         [
+            *layers,
             (_UpstreamCore, lambda _old: MultiScaleDeformableAttention(backend=backend)),
             (
                 _UpstreamM2F,

@@ -17,6 +17,7 @@ from torch import Tensor, nn
 from ..core.runtime import Method as MSDAMethod
 from ..core.sanitize import check_2power, check_msda_params
 from ..registry import Backend, MSDABackend
+from ._dropout import check_dropout, drop_and_add
 
 __all__ = ["MSDAMethod", "MultiScaleDeformAttn2d"]
 
@@ -63,6 +64,10 @@ class MultiScaleDeformAttn2d(nn.Module):
     chunk_step
         Passed to a pinned backend, for the reference's signature; the HIP kernels
         take the whole batch at once.
+    dropout
+        Probability with which the output's elements are dropped in training
+        (:data:`~deformops_amd.registry.dropout`), before a residual is added. The
+        reference's layer has none.
 
     Raises
     ------
@@ -91,6 +96,7 @@ class MultiScaleDeformAttn2d(nn.Module):
         method: MSDAMethod | str = MSDAMethod.SOFTMAX,
         backend: Backend | MSDABackend | None = None,
         chunk_step: int = 128,
+        dropout: float = 0.0,
     ) -> None:
         super().__init__()
         check_msda_params(dim, num_heads, num_levels, num_points)
@@ -102,6 +108,7 @@ class MultiScaleDeformAttn2d(nn.Module):
         self.method = MSDAMethod(method)
         self.backend = backend
         self.chunk_step = chunk_step
+        self.dropout = check_dropout(dropout)
         samples = num_heads * num_levels * num_points
         self.proj_offset = nn.Linear(dim, 2 * samples)
         self.proj_weights = nn.Linear(dim, samples)
@@ -180,6 +187,9 @@ class MultiScaleDeformAttn2d(nn.Module):
         spatial_shapes: Tensor,
         level_start_index: Tensor,
         padding_mask: Tensor | None = None,
+        *,
+        residual: Tensor | None = None,
+        seed: int | Tensor | None = None,
     ) -> Tensor:
         """Attend ``v`` at places predicted from ``q``.
 
@@ -201,6 +211,10 @@ class MultiScaleDeformAttn2d(nn.Module):
         padding_mask
             Boolean ``(B, N)``, ``True`` at padded tokens, whose projected values are
             zeroed; or ``None``.
+        residual
+            ``(B, Q, dim_output)``, added to the (dropped) output; or ``None``.
+        seed
+            The dropout's seed; ``None`` draws one from torch's CPU generator.
 
         Returns
         -------
@@ -225,10 +239,11 @@ class MultiScaleDeformAttn2d(nn.Module):
             if self.backend is not None:
                 options["chunk_step"] = self.chunk_step
             out = msda(value, spatial_shapes, level_start_index, loc, weights, **options)
-        return self.proj_output(out)
+        return drop_and_add(self.proj_output(out), self.dropout, training=self.training, seed=seed, residual=residual)
 
     def extra_repr(self) -> str:
         return (
             f"dim={self.dim}, num_heads={self.num_heads}, num_levels={self.num_levels}, "
             f"num_points={self.num_points}, method={self.method.value}"
+            + (f", dropout={self.dropout}" if self.dropout else "")
         )
