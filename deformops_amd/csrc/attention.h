@@ -44,32 +44,42 @@ typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLowest = -INFINITY;
 
+template <int V> using Const = std::integral_constant<int, V>;
+
 enum MaskKind { kNoMask = 0, kBoolMask = 1, kFloatMask = 2 };
 
+// Rows of channels in memory: element strides of the image, the row and the head. Every row the
+// kernels read is aligned to 16 bytes and holds Dp channels (zeros past D); a call whose tensors
+// are not like that is packed first.
+struct Rows {
+  const void* at;
+  int64_t batch, row, head;
+};
+
 struct Args {
-  const void *q, *k, *v;
-  int64_t q_batch, q_row, q_head, k_batch, k_row, k_head, v_batch, v_row, v_head;
+  Rows q, k, v;
   const void* mask;
   int64_t mask_batch, mask_head, mask_row, mask_key;
   int mask_type;    // element type of a float mask
   bool mask_quads;  // four keys of a row lie side by side, aligned to their size
+  bool mask_words;  // 16 of them
   bool mask_of_keys;  // a bool mask that is one for all rows and heads: it removes states
   const void* lengths;
   bool lengths_i64;
   void* out;
-  float2* stats;  // (m, log2 l) of each row, m = +inf for a row without keys
+  float2* stats;  // [B][H][Q]: (m, log2 l) of each row, m = +inf for a row without keys
   int B, Q, S, K, G, D;
+  int Dp;      // D, rounded up to 16 bytes
   uint32_t R;  // rows of one (image, key head): Q * G
   float scale;
-  bool vector;  // operand rows may be read in 16-byte pieces
-  bool out_vector;
+  bool out_vector;  // results may be written four channels at a time
   int splits;
   float* part;         // [splits][B * K][R][D] unnormalized sums of each split
   float2* part_stats;  // [splits][B * K][R]
   // Backward.
-  const void* grad_out;
+  Rows o, go;
   const float2* row_stats;
-  float* delta;  // [B * K][R]
+  float* delta;  // [B][H][Q]
   void *grad_q, *grad_k, *grad_v;
   int row_splits;
   float* part_k;  // [row_splits][B][S][K][D]
@@ -80,10 +90,17 @@ struct Args {
 // Matrix products of one wave.
 
 // Precision of a 16-bit operand made from fp32 scores: p and ds are rounded to the operands'
-// type (bf16 2^-9, f16 2^-12 relative). f16 has 5 exponent bits: p is scaled by 2^14, so
-// that weights down to 2^-28 stay normal, and ds by a running power of two for each lane
-// (Scaled below).
+// type (bf16 2^-9, f16 2^-12 relative). f16 has 5 exponent bits: the backward scales p by 2^14,
+// so that weights down to 2^-28 stay normal, and ds by a running power of two for each lane
+// (Scaled below). The forward's weights exp2(x - m) are scaled by 2^9.
 template <typename T> constexpr float kWeightBits = std::is_same_v<T, f16_t> ? 14.0f : 0.0f;
+template <typename T> constexpr float kForwardBits = std::is_same_v<T, f16_t> ? 9.0f : 0.0f;
+
+// The forward's running maximum stays where it is until a score passes it by this many powers
+// of two: with random scores every tile has a row whose maximum moves by a little, and each
+// move costs a multiplication of all sums. Weights then reach 2^8 (f16: 2^5 2^9 = 2^14, in its
+// range), in a sum and a product that are as exact for them.
+template <typename T> constexpr float kSlack = std::is_same_v<T, f16_t> ? 5.0f : 8.0f;
 
 template <typename T> struct Mma;
 
@@ -126,20 +143,25 @@ template <> struct Mma<float> {
   }
 };
 
-// A tile of rows in LDS, DP channels each, in 16-byte pieces. The pieces of a row change
-// places by an exclusive or with the row's number, so that neighbouring rows' equal pieces
-// lie in different banks.
+// A tile of rows in LDS, DP channels each, in 16-byte pieces that change places within their row
+// by an exclusive or with bits of the row's number. LDS serves 64 banks (256 bytes) a cycle: 16
+// lanes of a row operand's read (one piece of 16 rows), or 32 lanes of a turning read (4
+// neighbouring pieces of 4 rows, 8 bytes a lane), have to lie in different sixteenths of 256
+// bytes. Measured on reads of both kinds: 540 and 300-320 bytes/ns a CU with these patterns,
+// 300 and 150 with `row & 7`.
 template <typename T, int DP> struct Tile {
   static constexpr int kPieces = DP * int(sizeof(T)) / 16;
   static constexpr int kRowBytes = kPieces * 16;
 
   static __device__ int offset(int row, int piece) {
     int turn;
-    if constexpr (kPieces % 8 == 0)
-      turn = row & 7;
-    else if constexpr (kPieces == 4)
-      turn = (row >> 1) & 3;
-    else
+    if constexpr (sizeof(T) == 4)  // single channels of rows r and r + 4 are read together
+      turn = kPieces % 16 == 0 ? (row & 3) | ((row & 4) << 1) | ((row & 8) >> 1) : row & 7;
+    else if constexpr (kPieces == 16)
+      turn = ((row & 3) << 2) | ((row >> 2) & 3);
+    else if constexpr (kPieces == 8)
+      turn = ((row & 2) << 1) | ((row >> 2) & 3);
+    else  // 4 or 12: rows r .. r + 3 differ in their sixteenths already
       turn = (row >> 2) & 3;
     return row * kRowBytes + ((piece ^ turn) << 4);
   }
@@ -185,18 +207,10 @@ template <typename T, int DP> __device__ inline u32x4 row_piece(const char* tile
   return *reinterpret_cast<const u32x4*>(tile + Tile<T, DP>::offset(row + lane % 32, 2 * step + lane / 32));
 }
 
-// 16 bytes of a row in memory, from channel c; zero past D.
-template <typename T> __device__ inline u32x4 load_piece(const T* row, int c, int D, bool vector) {
-  constexpr int N = 16 / int(sizeof(T));
+// 16 bytes of a row in memory, from channel c; zero past Dp.
+template <typename T> __device__ inline u32x4 load_piece(const T* row, int c, int Dp) {
   u32x4 out = {0, 0, 0, 0};
-  if (vector) {  // then D is a multiple of N
-    if (c < D) out = *reinterpret_cast<const u32x4*>(row + c);
-    return out;
-  }
-  T parts[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) parts[i] = c + i < D ? row[c + i] : T(0);
-  __builtin_memcpy(&out, parts, 16);
+  if (c < Dp) out = *reinterpret_cast<const u32x4*>(row + c);
   return out;
 }
 
@@ -219,32 +233,35 @@ __device__ inline int result_row(int r) { return 8 * (r / 4) + 4 * ((threadIdx.x
 // lane's column holds, so each lane keeps an exponent of its own, taken from the first values
 // (to 2^11 .. 2^12) and lowered, with the sums so far, when a later value would pass 2^15.
 template <typename T> struct Scaled {
+  static constexpr float power = 1.0f;
   template <int N> __device__ void fit(float (&)[16], f32x16 (&)[N]) {}
-  __device__ float undo(float v) const { return v; }
+  __device__ float undo() const { return 1.0f; }
 };
 template <> struct Scaled<f16_t> {
-  int e = 1 << 20;  // none yet
-  template <int N> __device__ void fit(float (&ds)[16], f32x16 (&acc)[N]) {
+  int e = 0;
+  bool set = false;
+  float power = 1.0f;  // 2^e, which the caller has put into ds
+  template <int N> __device__ __forceinline__ void fit(float (&ds)[16], f32x16 (&acc)[N]) {
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(ds[i]));
     top = half_max(top);
-    int bits = __builtin_amdgcn_frexp_expf(top);  // top = f 2^bits, f in [0.5, 1); 0 for 0, inf and NaN
-    const bool change = top > 0.0f && bits + e > 15;
+    const int bits = __builtin_amdgcn_frexp_expf(top);  // top = f 2^bits, f in [0.5, 1); 0 for 0, inf and NaN
+    const bool change = top > 0.0f && (bits > 15 || !set);
     if (__any(change)) {
-      const int next = change ? min(12 - bits, 120) : e;
-      const int by = e == (1 << 20) ? 0 : next - e;  // the sums are zero before the first
+      const int by = change ? min(12 - bits, 120 - e) : 0;
 #pragma unroll
       for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[n][i] = ldexpf(acc[n][i], by);
-      e = next;
-    }
-    const int by = e == (1 << 20) ? 0 : e;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) ds[i] = ldexpf(ds[i], by);
+      for (int i = 0; i < 16; ++i) ds[i] = ldexpf(ds[i], by);
+      e += by;
+      power = ldexpf(1.0f, e);
+      set |= change;
+    }
   }
-  __device__ float undo(float v) const { return ldexpf(v, e == (1 << 20) ? 0 : -e); }
+  __device__ float undo() const { return ldexpf(1.0f, -e); }
 };
 
 // ---------------------------------------------------------------------------
@@ -264,29 +281,33 @@ __device__ inline float float_mask(const Args& a, int64_t at) {
 }
 __device__ inline bool bool_mask(const Args& a, int64_t at) { return static_cast<const uint8_t*>(a.mask)[at] != 0; }
 
-// Bit r: whether the mask leaves the key of result row r (32 keys from `key`) to the row whose
-// first mask element is `at`. Keys at or past `limit` count as left out.
-__device__ inline uint32_t bool_bits(const Args& a, int64_t at, int key, int limit) {
-  uint32_t bits = 0;
+// A bool mask's bytes for the 16 result rows (32 keys from `key`) of the row whose first mask
+// element is `at`: four words, result row r in byte r % 4 of word r / 4. Keys at or past `limit`
+// are left out.
+struct MaskBytes {
+  uint32_t word[4];
+  __device__ bool any() const { return (word[0] | word[1] | word[2] | word[3]) != 0; }
+  __device__ bool on(int r) const { return ((word[r / 4] >> (8 * (r % 4))) & 0xff) != 0; }
+};
+__device__ __forceinline__ MaskBytes mask_bytes(const Args& a, int64_t at, int key, int limit) {
+  MaskBytes out = {};
   const int half = (threadIdx.x % kWave) / 32;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const int k0 = key + 8 * g + 4 * half;
     if (a.mask_quads && k0 + 4 <= limit) {
-      const uint32_t four = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.mask) + at + k0);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) bits |= uint32_t(((four >> (8 * i)) & 0xff) != 0) << (4 * g + i);
+      out.word[g] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.mask) + at + k0);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (k0 + i < limit) bits |= uint32_t(bool_mask(a, at + int64_t(k0 + i) * a.mask_key)) << (4 * g + i);
+        if (k0 + i < limit) out.word[g] |= uint32_t(bool_mask(a, at + int64_t(k0 + i) * a.mask_key)) << (8 * i);
     }
   }
-  return bits;
+  return out;
 }
 
 // The additive mask of the 16 result rows, -inf at or past `limit`.
-__device__ inline void float_masks(const Args& a, int64_t at, int key, int limit, float (&out)[16]) {
+__device__ __forceinline__ void float_masks(const Args& a, int64_t at, int key, int limit, float (&out)[16]) {
   const int half = (threadIdx.x % kWave) / 32;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
@@ -315,44 +336,73 @@ __device__ inline RowOf row_of(const Args& a, int kv, uint32_t r) {
 __device__ inline int64_t mask_row_at(const Args& a, int b, RowOf o) {
   return b * a.mask_batch + int64_t(o.head) * a.mask_head + int64_t(o.query) * a.mask_row;
 }
+template <typename T> __device__ inline const T* row_at(const Rows& rows, int b, RowOf o) {
+  return static_cast<const T*>(rows.at) + b * rows.batch + int64_t(o.query) * rows.row + int64_t(o.head) * rows.head;
+}
+__device__ inline int64_t stat_at(const Args& a, int b, RowOf o) {
+  return (int64_t(b) * (a.K * a.G) + o.head) * a.Q + o.query;
+}
 
 // ---------------------------------------------------------------------------
 // Staging: tile rows from memory to LDS through registers, so that the next tile's loads are
-// under way while this one is worked on.
+// under way while this one is worked on. Buffer loads answer zero outside their range, which
+// is how rows past the last and channels past Dp become zeros.
 
-template <typename T, int DP, int ROWS, int THREADS> struct Stage {
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr uint32_t kOutside = 0x80000000u;  // past every range, which is at most 2^31 bytes
+
+template <typename T> __device__ inline const T* uniform(const T* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(v)), hi = __builtin_amdgcn_readfirstlane(uint32_t(v >> 32));
+  return reinterpret_cast<const T*>((uint64_t(hi) << 32) | lo);
+}
+
+template <typename T, int DP, int ROWS> struct Stage {
   static constexpr int kPieces = Tile<T, DP>::kPieces;
-  static constexpr int kEach = ROWS * kPieces / THREADS;
-  static_assert(ROWS * kPieces % THREADS == 0);
-  static constexpr int kBytes = ROWS * Tile<T, DP>::kRowBytes;
+  static constexpr int kEach = ROWS * kPieces / kThreads;
+  static_assert(ROWS * kPieces % kThreads == 0);
   u32x4 hold[kEach];
+  uint32_t from[kEach];
+  uint32_t stride;  // bytes
 
-  // `row_at(row)` is the row's address, or null for a row of zeros.
-  template <typename F> __device__ void load(F row_at, int D, bool vector) {
+  static __device__ int row(int i) { return (i * kThreads + int(threadIdx.x)) / kPieces; }
+  static __device__ int piece(int i) { return (i * kThreads + int(threadIdx.x)) % kPieces; }
+
+  __device__ void plan(int64_t row_stride, int Dp) {
+    stride = uint32_t(row_stride) * uint32_t(sizeof(T));
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int n = i * THREADS + int(threadIdx.x), row = n / kPieces, piece = n % kPieces;
-      const T* p = row_at(row);
-      const u32x4 zero = {0, 0, 0, 0};
-      hold[i] = p ? load_piece(p, piece * (16 / int(sizeof(T))), D, vector) : zero;
-    }
+    for (int i = 0; i < kEach; ++i)
+      from[i] = piece(i) * (16 / int(sizeof(T))) < Dp ? uint32_t(row(i)) * stride + uint32_t(piece(i)) * 16 : kOutside;
   }
-  __device__ void store(char* tile) const {
+  // ROWS rows from `base` (the same for all lanes), of which `left` exist; `kept(row)` whether
+  // a row is read.
+  template <typename F> __device__ __forceinline__ void load(const T* base, int left, F kept) {
+    const uint32_t bytes = __builtin_amdgcn_readfirstlane(uint32_t(left < ROWS ? left : ROWS) * stride);
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(uniform(base)), 0, bytes, 0x00027000);
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int n = i * THREADS + int(threadIdx.x);
-      *reinterpret_cast<u32x4*>(tile + Tile<T, DP>::offset(n / kPieces, n % kPieces)) = hold[i];
-    }
+    for (int i = 0; i < kEach; ++i)
+      hold[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, kept(row(i)) ? from[i] : kOutside, 0, 0);
+  }
+  __device__ __forceinline__ void store(char* tile) const {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) *reinterpret_cast<u32x4*>(tile + Tile<T, DP>::offset(row(i), piece(i))) = hold[i];
   }
 };
+
+struct All {
+  __device__ bool operator()(int) const { return true; }
+};
+
+// Two waves of a SIMD hide each other's waits where their registers allow it (256 each).
+template <typename T, int DP> constexpr int kForwardWaves = sizeof(T) == 4 && DP > 64 ? 1 : 2;
+template <typename T, int DP> constexpr int kGradQWaves = DP * int(sizeof(T)) <= (sizeof(T) == 4 ? 128 : 192) ? 2 : 1;
+template <typename T, int DP> constexpr int kGradStatesWaves = DP * int(sizeof(T)) <= 128 ? 2 : 1;
 
 // ---------------------------------------------------------------------------
 // Forward. A workgroup has 4 waves: WR of them along the rows (32 each), 4 / WR along the keys
 // of a tile (KB blocks of 32 each), whose partial sums meet in LDS at the end. Splits of the
 // key axis leave unnormalized sums, which combine_kernel joins.
-
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * kWave;
 
 template <typename T, int DP, int WR> struct ForwardShape {
   static constexpr int WK = kWaves / WR;
@@ -360,7 +410,7 @@ template <typename T, int DP, int WR> struct ForwardShape {
   static constexpr int kRows = 32 * WR;
   static constexpr int kKeys = 32 * KB * WK;
   static constexpr int kTile = kKeys * Tile<T, DP>::kRowBytes;
-  static constexpr int kBuffers = 4 * kTile <= 128 * 1024 ? 2 : 1;
+  static constexpr int kBuffers = 4 * kTile <= (kForwardWaves<T, DP> == 2 ? 80 : 128) * 1024 ? 2 : 1;
   static constexpr int kJoin = WK > 1 ? WK * 32 * WR * (DP + 2) * 4 : 0;
   static constexpr int kLds = std::max(2 * kBuffers * kTile, kJoin);
 };
@@ -402,8 +452,67 @@ template <int NB> struct Softmax {
   }
 };
 
+// What a workgroup of the walks over the keys works on.
+template <typename Shape> struct KeyWalk {
+  int b, kv, bk, split, first, last, states;
+  uint32_t row_tile;
+
+  __device__ explicit KeyWalk(const Args& a) {
+    const uint32_t row_tiles = (a.R + Shape::kRows - 1) / Shape::kRows;
+    uint32_t id = xcd_order(blockIdx.x, gridDim.x);
+    row_tile = id % row_tiles;
+    id /= row_tiles;
+    split = int(id % uint32_t(a.splits));
+    bk = int(id / uint32_t(a.splits));
+    b = bk / a.K;
+    kv = bk % a.K;
+    states = __builtin_amdgcn_readfirstlane(states_of(a, b));
+    const int tiles = (states + Shape::kKeys - 1) / Shape::kKeys;
+    first = int(int64_t(tiles) * split / a.splits);
+    last = int(int64_t(tiles) * (split + 1) / a.splits);
+  }
+};
+
+// The tiles of keys and values on their way to LDS, and a bool mask's bytes of the next tile.
+template <typename T, int DP, int MASK, typename Shape> struct KeyStage {
+  static constexpr int KB = Shape::KB;
+  const Args& a;
+  const KeyWalk<Shape>& w;
+  Stage<T, DP, Shape::kKeys> k, v;
+  const T *k_base, *v_base;
+  int64_t mask_at;
+  int local;  // this wave's first key in a tile
+  MaskBytes next[KB];
+
+  __device__ KeyStage(const Args& args, const KeyWalk<Shape>& walk, int64_t mask, int first_key)
+      : a(args), w(walk), mask_at(mask), local(first_key) {
+    k.plan(a.k.row, a.Dp);
+    v.plan(a.v.row, a.Dp);
+    k_base = static_cast<const T*>(a.k.at) + w.b * a.k.batch + w.kv * a.k.head;
+    v_base = static_cast<const T*>(a.v.at) + w.b * a.v.batch + w.kv * a.v.head;
+  }
+  __device__ __forceinline__ void load(int tile) {
+    const int key = tile * Shape::kKeys, left = w.states - key;
+    const T *ks = k_base + int64_t(key) * a.k.row, *vs = v_base + int64_t(key) * a.v.row;
+    if (MASK == kBoolMask && a.mask_of_keys) {  // removed states are read as zeros
+      auto kept = [&](int row) {
+        return row < left && bool_mask(a, w.b * a.mask_batch + int64_t(key + row) * a.mask_key);
+      };
+      k.load(ks, left, kept);
+      v.load(vs, left, kept);
+    } else {
+      k.load(ks, left, All());
+      v.load(vs, left, All());
+    }
+    if constexpr (MASK == kBoolMask) {
+#pragma unroll
+      for (int n = 0; n < KB; ++n) next[n] = mask_bytes(a, mask_at, key + local + 32 * n, w.states);
+    }
+  }
+};
+
 template <typename T, int DP, int MASK, int WR>
-__global__ __launch_bounds__(kThreads) void attention_forward_kernel(const Args a) {
+__global__ __launch_bounds__(kThreads, (kForwardWaves<T, DP>)) void attention_forward_kernel(const Args a) {
   using Shape = ForwardShape<T, DP, WR>;
   using TileT = Tile<T, DP>;
   constexpr int KB = Shape::KB, NB = DP / 32, kSteps = TileT::kPieces / 2, kKeys = Shape::kKeys;
@@ -411,103 +520,69 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(const Args 
 
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int wr = wave % WR, wk = wave / WR;
-  const uint32_t row_tiles = (a.R + Shape::kRows - 1) / Shape::kRows;
-  uint32_t id = xcd_order(blockIdx.x, gridDim.x);
-  const uint32_t row_tile = id % row_tiles;
-  id /= row_tiles;
-  const int split = int(id % uint32_t(a.splits));
-  const int bk = int(id / uint32_t(a.splits));
-  const int b = bk / a.K, kv = bk % a.K;
-
-  const uint32_t r = row_tile * Shape::kRows + 32 * wr + lane % 32;
+  const KeyWalk<Shape> w(a);
+  const uint32_t r = w.row_tile * Shape::kRows + 32 * wr + lane % 32;
   const bool live = r < a.R;
-  const RowOf mine = row_of(a, kv, live ? r : a.R - 1);
+  const RowOf mine = row_of(a, w.kv, live ? r : a.R - 1);
+  int64_t mask_at = 0;
+  if constexpr (MASK != kNoMask) mask_at = mask_row_at(a, w.b, mine);
+  const int local = 32 * KB * wk;
+  KeyStage<T, DP, MASK, Shape> stage(a, w, mask_at, local);
+  if (w.first < w.last) stage.load(w.first);
 
   u32x4 q[kSteps];
   {
-    const T* row = static_cast<const T*>(a.q) + b * a.q_batch + int64_t(mine.query) * a.q_row + mine.head * a.q_head;
+    const T* row = row_at<T>(a.q, w.b, mine);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const u32x4 zero = {0, 0, 0, 0};
-      q[s] = live ? load_piece(row, (2 * s + lane / 32) * (16 / int(sizeof(T))), a.D, a.vector) : zero;
+      q[s] = live ? load_piece(row, (2 * s + lane / 32) * (16 / int(sizeof(T))), a.Dp) : zero;
     }
   }
-  int64_t mask_at = 0;
-  if constexpr (MASK != kNoMask) mask_at = mask_row_at(a, b, mine);
-
-  // This split's keys: whole tiles of this image's states.
-  const int states = states_of(a, b);
-  const int tiles = (states + kKeys - 1) / kKeys;
-  const int first = int(int64_t(tiles) * split / a.splits), last = int(int64_t(tiles) * (split + 1) / a.splits);
-
-  const T* k_base = static_cast<const T*>(a.k) + b * a.k_batch + kv * a.k_head;
-  const T* v_base = static_cast<const T*>(a.v) + b * a.v_batch + kv * a.v_head;
-  auto kept = [&](int key) {  // a state that the lengths or a mask of keys removes is read as zero
-    if (key >= states) return false;
-    if constexpr (MASK == kBoolMask)
-      if (a.mask_of_keys) return bool_mask(a, b * a.mask_batch + int64_t(key) * a.mask_key);
-    return true;
-  };
-  Stage<T, DP, kKeys, kThreads> k_stage, v_stage;
-  auto load = [&](int tile) {
-    k_stage.load([&](int row) -> const T* {
-      const int key = tile * kKeys + row;
-      return kept(key) ? k_base + int64_t(key) * a.k_row : nullptr;
-    }, a.D, a.vector);
-    v_stage.load([&](int row) -> const T* {
-      const int key = tile * kKeys + row;
-      return kept(key) ? v_base + int64_t(key) * a.v_row : nullptr;
-    }, a.D, a.vector);
-  };
 
   Softmax<NB> soft;
   const float factor = MASK == kFloatMask ? a.scale : a.scale * kLog2e;
-  if (first < last) load(first);
-  for (int tile = first; tile < last; ++tile) {
-    char* k_tile = lds + ((tile - first) % Shape::kBuffers) * 2 * Shape::kTile;
-    char* v_tile = k_tile + Shape::kTile;
-    if (Shape::kBuffers == 1 && tile > first) __syncthreads();
-    k_stage.store(k_tile);
-    v_stage.store(v_tile);
-    __syncthreads();
-    if (tile + 1 < last) load(tile + 1);
+  constexpr float kStay = MASK == kFloatMask ? kSlack<T> / kLog2e : kSlack<T>;
 
-    const int key0 = tile * kKeys + 32 * KB * wk;  // this wave's keys
-    const int local = 32 * KB * wk;
-    uint32_t bits[KB];
-    if constexpr (MASK == kBoolMask) {
-      uint32_t any = 0;
+  auto step = [&](int tile, auto buffer) __attribute__((always_inline)) {
+    char* k_tile = lds + decltype(buffer)::value * 2 * Shape::kTile;
+    char* v_tile = k_tile + Shape::kTile;
+    if (Shape::kBuffers == 1 && tile > w.first) __syncthreads();
+    stage.k.store(k_tile);
+    stage.v.store(v_tile);
+    MaskBytes mask[KB];
 #pragma unroll
-      for (int n = 0; n < KB; ++n) any |= bits[n] = bool_bits(a, mask_at, key0 + 32 * n, states);
-      if (!__any(any != 0 && live)) continue;
+    for (int n = 0; n < KB; ++n) mask[n] = stage.next[n];
+    __syncthreads();
+    if (tile + 1 < w.last) stage.load(tile + 1);
+
+    const int key0 = tile * kKeys + local;  // this wave's keys
+    if constexpr (MASK == kBoolMask) {
+      bool any = false;
+#pragma unroll
+      for (int n = 0; n < KB; ++n) any |= mask[n].any();
+      if (!__any(any && live)) return;
     }
     float x[KB][16];
 #pragma unroll
     for (int n = 0; n < KB; ++n) {
+      float add[16];
+      if constexpr (MASK == kFloatMask) float_masks(a, mask_at, key0 + 32 * n, w.states, add);
       f32x16 s = {};
 #pragma unroll
       for (int t = 0; t < kSteps; ++t) s = Mma<T>::rows(row_piece<T, DP>(k_tile, local + 32 * n, t), q[t], s);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[n][i] = s[i];
-    }
-    if constexpr (MASK == kBoolMask) {
-#pragma unroll
-      for (int n = 0; n < KB; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[n][i] = (bits[n] >> i) & 1 ? x[n][i] : kLowest;
-    } else if constexpr (MASK == kFloatMask) {
-#pragma unroll
-      for (int n = 0; n < KB; ++n) {
-        float add[16];
-        float_masks(a, mask_at, key0 + 32 * n, states, add);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[n][i] = add[i] == kLowest ? kLowest : fmaf(x[n][i], factor, add[i]);
+      for (int i = 0; i < 16; ++i) {
+        x[n][i] = s[i];
+        if constexpr (MASK == kBoolMask) x[n][i] = mask[n].on(i) ? s[i] : kLowest;
+        if constexpr (MASK == kFloatMask) x[n][i] = add[i] == kLowest ? kLowest : fmaf(s[i], factor, add[i]);
       }
-    } else if (key0 + 32 * KB > states) {
+    }
+    if (MASK == kNoMask && key0 + 32 * KB > w.states) {
 #pragma unroll
       for (int n = 0; n < KB; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[n][i] = key0 + 32 * n + result_row(i) < states ? x[n][i] : kLowest;
+        for (int i = 0; i < 16; ++i) x[n][i] = key0 + 32 * n + result_row(i) < w.states ? x[n][i] : kLowest;
     }
     float top = kLowest;
 #pragma unroll
@@ -516,29 +591,33 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(const Args 
       for (int i = 0; i < 16; ++i) top = fmaxf(top, x[n][i]);
     top = half_max(top);
     if constexpr (MASK != kFloatMask) top *= factor;
-    if (__any(top > soft.m)) {
+    if (__any(top > soft.m + kStay)) {
       const float m = fmaxf(soft.m, top);
       const float by = m == soft.m ? 0.0f : soft.m - m;  // 0 too where both are -inf
       soft.rescale(__builtin_amdgcn_exp2f(MASK == kFloatMask ? by * kLog2e : by));
       soft.m = m;
     }
     const float base = soft.m == kLowest ? 0.0f : soft.m;  // all -inf: every weight is exp2(-inf)
+    const float shift = kForwardBits<T> - base;
     float sum = 0.0f;
 #pragma unroll
     for (int n = 0; n < KB; ++n) {
       float p[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float y = MASK == kFloatMask ? fmaf(x[n][i] - base, kLog2e, kWeightBits<T>)
-                                           : fmaf(x[n][i], factor, kWeightBits<T> - base);
+        const float y = MASK == kFloatMask ? fmaf(x[n][i] - base, kLog2e, kForwardBits<T>) : fmaf(x[n][i], factor, shift);
         p[i] = __builtin_amdgcn_exp2f(y);
         sum += p[i];
       }
-      const auto w = Mma<T>::weights(p);
+      const auto weights = Mma<T>::weights(p);
 #pragma unroll
-      for (int c = 0; c < NB; ++c) soft.acc[c] = accumulate<T, DP>(v_tile, local + 32 * n, c, w, soft.acc[c]);
+      for (int c = 0; c < NB; ++c) soft.acc[c] = accumulate<T, DP>(v_tile, local + 32 * n, c, weights, soft.acc[c]);
     }
     soft.l += sum;
+  };
+  for (int tile = w.first; tile < w.last; tile += 2) {
+    step(tile, Const<0>());
+    if (tile + 1 < w.last) step(tile + 1, Const<Shape::kBuffers - 1>());
   }
 
   // Join the waves that share rows: each leaves its sums in LDS, wave 0 of them adds.
@@ -576,7 +655,7 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(const Args 
   if (!live) return;
 
   if (a.splits > 1) {
-    const int64_t at = (int64_t(split) * a.B * a.K + bk) * a.R + r;
+    const int64_t at = (int64_t(w.split) * a.B * a.K + w.bk) * a.R + r;
     if (lane < 32) a.part_stats[at] = float2{soft.m, soft.l};
     float* part = a.part + at * a.D;
 #pragma unroll
@@ -591,9 +670,9 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(const Args 
   }
   const float inverse = soft.m == kLowest ? 0.0f : 1.0f / soft.l;
   if (a.stats && lane < 32)
-    a.stats[int64_t(bk) * a.R + r] = soft.m == kLowest ? float2{INFINITY, 0.0f}
-                                                       : float2{soft.m, log2f(soft.l) - kWeightBits<T>};
-  T* out = static_cast<T*>(a.out) + ((int64_t(b) * a.Q + mine.query) * (a.K * a.G) + mine.head) * a.D;
+    a.stats[stat_at(a, w.b, mine)] = soft.m == kLowest ? float2{INFINITY, 0.0f}
+                                                       : float2{soft.m, log2f(soft.l) - kForwardBits<T>};
+  T* out = static_cast<T*>(a.out) + ((int64_t(w.b) * a.Q + mine.query) * (a.K * a.G) + mine.head) * a.D;
 #pragma unroll
   for (int c = 0; c < NB; ++c)
 #pragma unroll
@@ -606,27 +685,30 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(const Args 
     }
 }
 
-// Joins the splits of the forward: one thread per row and four channels.
-template <typename T> __global__ __launch_bounds__(256) void attention_combine_kernel(const Args a, bool natural) {
-  const int quads = (a.D + 3) / 4;
+// Joins the splits of the forward. A row has `lanes` lanes (a power of two) of four channels
+// each, and 64 / lanes of them in a wave share its splits, so that few rows of many splits do
+// not wait for one lane's loads in turn.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_combine_kernel(const Args a, int lanes, bool natural) {
   const int64_t rows = int64_t(a.B) * a.K * a.R;
-  const int64_t n = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (n >= rows * quads) return;
-  const int64_t row = n / quads;
-  const int d = int(n % quads) * 4;
+  const int64_t row = int64_t(blockIdx.x) * kWaves + threadIdx.x / kWave;
+  if (row >= rows) return;  // whole waves
+  const int lane = threadIdx.x % kWave, share = lane / lanes, shares = kWave / lanes;
+  const int d = (lane % lanes) * 4, left = a.D - d;
   const float unit = natural ? kLog2e : 1.0f;
   float m = kLowest;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_stats[s * rows + row].x);
+  for (int s = lane; s < a.splits; s += kWave) m = fmaxf(m, a.part_stats[s * rows + row].x);
+  for (int by = 32; by; by /= 2) m = fmaxf(m, __shfl_xor(m, by));
   float l = 0.0f, v[4] = {};
-  const int left = a.D - d;
-  for (int s = 0; s < a.splits; ++s) {
+#pragma unroll 4
+  for (int s = share; s < a.splits; s += shares) {
     const float2 st = a.part_stats[s * rows + row];
-    if (st.x == kLowest) continue;
-    const float f = st.x == m ? 1.0f : __builtin_amdgcn_exp2f((st.x - m) * unit);
+    const float f = st.x == kLowest ? 0.0f : st.x == m ? 1.0f : __builtin_amdgcn_exp2f((st.x - m) * unit);
     l = fmaf(st.y, f, l);
     const float* p = a.part + (s * rows + row) * a.D + d;
     if (a.D % 4 == 0) {
-      const f32x4 four = *reinterpret_cast<const f32x4*>(p);
+      f32x4 four = {0, 0, 0, 0};
+      if (left > 0) four = *reinterpret_cast<const f32x4*>(p);
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = fmaf(four[i], f, v[i]);
     } else {
@@ -635,6 +717,12 @@ template <typename T> __global__ __launch_bounds__(256) void attention_combine_k
         if (i < left) v[i] = fmaf(p[i], f, v[i]);
     }
   }
+  for (int by = lanes; by < kWave; by *= 2) {
+    l += __shfl_xor(l, by);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += __shfl_xor(v[i], by);
+  }
+  if (share > 0) return;
   const float inverse = m == kLowest ? 0.0f : 1.0f / l;
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] *= inverse;
@@ -642,8 +730,8 @@ template <typename T> __global__ __launch_bounds__(256) void attention_combine_k
   const RowOf o = row_of(a, bk % a.K, uint32_t(row % a.R));
   T* out = static_cast<T*>(a.out) + ((int64_t(b) * a.Q + o.query) * (a.K * a.G) + o.head) * a.D;
   store_four(out + d, v, left, a.out_vector);
-  if (a.stats && d == 0)
-    a.stats[row] = m == kLowest ? float2{INFINITY, 0.0f} : float2{m, log2f(l) - kWeightBits<T>};
+  if (a.stats && lane == 0)
+    a.stats[stat_at(a, b, o)] = m == kLowest ? float2{INFINITY, 0.0f} : float2{m, log2f(l) - kForwardBits<T>};
 }
 
 // ---------------------------------------------------------------------------
@@ -651,7 +739,7 @@ template <typename T> __global__ __launch_bounds__(256) void attention_combine_k
 // It also leaves delta_i = do_i . o_i of its rows for the states' kernel.
 
 template <typename T, int DP, int MASK, int WR>
-__global__ __launch_bounds__(kThreads) void attention_grad_q_kernel(const Args a) {
+__global__ __launch_bounds__(kThreads, (kGradQWaves<T, DP>)) void attention_grad_q_kernel(const Args a) {
   using Shape = ForwardShape<T, DP, WR>;
   using TileT = Tile<T, DP>;
   constexpr int KB = Shape::KB, NB = DP / 32, kSteps = TileT::kPieces / 2, kKeys = Shape::kKeys;
@@ -660,30 +748,27 @@ __global__ __launch_bounds__(kThreads) void attention_grad_q_kernel(const Args a
 
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int wr = wave % WR, wk = wave / WR;
-  const uint32_t row_tiles = (a.R + Shape::kRows - 1) / Shape::kRows;
-  uint32_t id = xcd_order(blockIdx.x, gridDim.x);
-  const uint32_t row_tile = id % row_tiles;
-  id /= row_tiles;
-  const int split = int(id % uint32_t(a.splits));
-  const int bk = int(id / uint32_t(a.splits));
-  const int b = bk / a.K, kv = bk % a.K;
-
-  const uint32_t r = row_tile * Shape::kRows + 32 * wr + lane % 32;
+  const KeyWalk<Shape> w(a);
+  const uint32_t r = w.row_tile * Shape::kRows + 32 * wr + lane % 32;
   const bool live = r < a.R;
-  const RowOf mine = row_of(a, kv, live ? r : a.R - 1);
-  const int64_t out_at = ((int64_t(b) * a.Q + mine.query) * (a.K * a.G) + mine.head) * a.D;
+  const RowOf mine = row_of(a, w.kv, live ? r : a.R - 1);
+  int64_t mask_at = 0;
+  if constexpr (MASK != kNoMask) mask_at = mask_row_at(a, w.b, mine);
+  const int local = 32 * KB * wk;
+  KeyStage<T, DP, MASK, Shape> stage(a, w, mask_at, local);
+  if (w.first < w.last) stage.load(w.first);
 
   u32x4 q[kSteps], go[kSteps];
   float delta = 0.0f;
   {
-    const T* row = static_cast<const T*>(a.q) + b * a.q_batch + int64_t(mine.query) * a.q_row + mine.head * a.q_head;
+    const T *q_row = row_at<T>(a.q, w.b, mine), *go_row = row_at<T>(a.go, w.b, mine), *o_row = row_at<T>(a.o, w.b, mine);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const int c = (2 * s + lane / 32) * N;
       const u32x4 zero = {0, 0, 0, 0};
-      q[s] = live ? load_piece(row, c, a.D, a.vector) : zero;
-      go[s] = live ? load_piece(static_cast<const T*>(a.grad_out) + out_at, c, a.D, a.out_vector) : zero;
-      const u32x4 o = live ? load_piece(static_cast<const T*>(a.out) + out_at, c, a.D, a.out_vector) : zero;
+      q[s] = live ? load_piece(q_row, c, a.Dp) : zero;
+      go[s] = live ? load_piece(go_row, c, a.Dp) : zero;
+      const u32x4 o = live ? load_piece(o_row, c, a.Dp) : zero;
       T x[N], y[N];
       __builtin_memcpy(x, &go[s], 16);
       __builtin_memcpy(y, &o, 16);
@@ -692,91 +777,69 @@ __global__ __launch_bounds__(kThreads) void attention_grad_q_kernel(const Args a
     }
     delta = half_sum(delta);
   }
-  const float2 stat = live ? a.row_stats[int64_t(bk) * a.R + r] : float2{INFINITY, 0.0f};
-  if (split == 0 && wk == 0 && live && lane < 32) a.delta[int64_t(bk) * a.R + r] = delta;
-  int64_t mask_at = 0;
-  if constexpr (MASK != kNoMask) mask_at = mask_row_at(a, b, mine);
-
-  const int states = states_of(a, b);
-  const int tiles = (states + kKeys - 1) / kKeys;
-  const int first = int(int64_t(tiles) * split / a.splits), last = int(int64_t(tiles) * (split + 1) / a.splits);
-  const T* k_base = static_cast<const T*>(a.k) + b * a.k_batch + kv * a.k_head;
-  const T* v_base = static_cast<const T*>(a.v) + b * a.v_batch + kv * a.v_head;
-  auto kept = [&](int key) {
-    if (key >= states) return false;
-    if constexpr (MASK == kBoolMask)
-      if (a.mask_of_keys) return bool_mask(a, b * a.mask_batch + int64_t(key) * a.mask_key);
-    return true;
-  };
-  Stage<T, DP, kKeys, kThreads> k_stage, v_stage;
-  auto load = [&](int tile) {
-    k_stage.load([&](int row) -> const T* {
-      const int key = tile * kKeys + row;
-      return kept(key) ? k_base + int64_t(key) * a.k_row : nullptr;
-    }, a.D, a.vector);
-    v_stage.load([&](int row) -> const T* {
-      const int key = tile * kKeys + row;
-      return kept(key) ? v_base + int64_t(key) * a.v_row : nullptr;
-    }, a.D, a.vector);
-  };
+  const float2 stat = live ? a.row_stats[stat_at(a, w.b, mine)] : float2{INFINITY, 0.0f};
+  if (w.split == 0 && wk == 0 && live && lane < 32) a.delta[stat_at(a, w.b, mine)] = delta;
 
   f32x16 acc[NB] = {};
   Scaled<T> scaled;
   const float factor = MASK == kFloatMask ? a.scale : a.scale * kLog2e;
   const float shift = kWeightBits<T> - (MASK == kFloatMask ? stat.y : stat.x + stat.y);
-  if (first < last) load(first);
-  for (int tile = first; tile < last; ++tile) {
-    char* k_tile = lds + ((tile - first) % Shape::kBuffers) * 2 * Shape::kTile;
+
+  auto step = [&](int tile, auto buffer) __attribute__((always_inline)) {
+    char* k_tile = lds + decltype(buffer)::value * 2 * Shape::kTile;
     char* v_tile = k_tile + Shape::kTile;
-    if (Shape::kBuffers == 1 && tile > first) __syncthreads();
-    k_stage.store(k_tile);
-    v_stage.store(v_tile);
+    if (Shape::kBuffers == 1 && tile > w.first) __syncthreads();
+    stage.k.store(k_tile);
+    stage.v.store(v_tile);
+    MaskBytes mask[KB];
+#pragma unroll
+    for (int n = 0; n < KB; ++n) mask[n] = stage.next[n];
     __syncthreads();
-    if (tile + 1 < last) load(tile + 1);
+    if (tile + 1 < w.last) stage.load(tile + 1);
 
 #pragma unroll
     for (int n = 0; n < KB; ++n) {
-      const int local = 32 * (KB * wk + n), key0 = tile * kKeys + local;
-      uint32_t bits = 0;
-      if constexpr (MASK == kBoolMask) {
-        bits = bool_bits(a, mask_at, key0, states);
-        if (!__any(bits != 0 && live)) continue;
-      }
+      const int here = local + 32 * n, key0 = tile * kKeys + here;
+      if constexpr (MASK == kBoolMask)
+        if (!__any(mask[n].any() && live)) continue;
+      float add[16];
+      if constexpr (MASK == kFloatMask) float_masks(a, mask_at, key0, w.states, add);
       f32x16 s = {}, dp = {};
 #pragma unroll
       for (int t = 0; t < kSteps; ++t) {
-        s = Mma<T>::rows(row_piece<T, DP>(k_tile, local, t), q[t], s);
-        dp = Mma<T>::rows(row_piece<T, DP>(v_tile, local, t), go[t], dp);
+        s = Mma<T>::rows(row_piece<T, DP>(k_tile, here, t), q[t], s);
+        dp = Mma<T>::rows(row_piece<T, DP>(v_tile, here, t), go[t], dp);
       }
-      float ds[16], add[16];
-      if constexpr (MASK == kFloatMask) float_masks(a, mask_at, key0, states, add);
+      float ds[16];
+      const float low = delta * scaled.power;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        bool on = true;
-        float y;
-        if constexpr (MASK == kFloatMask) {
-          on = add[i] != kLowest;
-          y = fmaf(fmaf(s[i], factor, add[i]) - stat.x, kLog2e, shift);
-        } else {
-          if constexpr (MASK == kBoolMask) on = (bits >> i) & 1;
-          else on = key0 + result_row(i) < states;
-          y = fmaf(s[i], factor, shift);
-        }
-        const float p = __builtin_amdgcn_exp2f(y);
-        ds[i] = on ? p * (dp[i] - delta) : 0.0f;
+        const float y = MASK == kFloatMask ? fmaf(fmaf(s[i], factor, add[i]) - stat.x, kLog2e, shift)
+                                           : fmaf(s[i], factor, shift);
+        ds[i] = __builtin_amdgcn_exp2f(y) * fmaf(dp[i], scaled.power, -low);
+        if constexpr (MASK == kBoolMask) ds[i] = mask[n].on(i) ? ds[i] : 0.0f;
+        if constexpr (MASK == kFloatMask) ds[i] = add[i] == kLowest ? 0.0f : ds[i];
+      }
+      if (MASK == kNoMask && key0 + 32 > w.states) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ds[i] = key0 + result_row(i) < w.states ? ds[i] : 0.0f;
       }
       scaled.fit(ds, acc);
-      const auto w = Mma<T>::weights(ds);
+      const auto weights = Mma<T>::weights(ds);
 #pragma unroll
-      for (int c = 0; c < NB; ++c) acc[c] = accumulate<T, DP>(k_tile, local, c, w, acc[c]);
+      for (int c = 0; c < NB; ++c) acc[c] = accumulate<T, DP>(k_tile, here, c, weights, acc[c]);
     }
+  };
+  for (int tile = w.first; tile < w.last; tile += 2) {
+    step(tile, Const<0>());
+    if (tile + 1 < w.last) step(tile + 1, Const<Shape::kBuffers - 1>());
   }
 
-  const float unit = a.scale * __builtin_amdgcn_exp2f(-kWeightBits<T>);
+  const float unit = a.scale * __builtin_amdgcn_exp2f(-kWeightBits<T>), undo = scaled.undo();
 #pragma unroll
   for (int c = 0; c < NB; ++c)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[c][i] = scaled.undo(acc[c][i]) * unit;
+    for (int i = 0; i < 16; ++i) acc[c][i] = acc[c][i] * undo * unit;
   if constexpr (Shape::WK > 1) {
     __syncthreads();
     float* mine_at = reinterpret_cast<float*>(lds) + wave * 32 * DP;
@@ -797,6 +860,7 @@ __global__ __launch_bounds__(kThreads) void attention_grad_q_kernel(const Args a
   if (!live) return;
   // A split's sums lie in grad_q's own order.
   const int64_t elements = int64_t(a.B) * a.Q * a.K * a.G * a.D;
+  const int64_t out_at = ((int64_t(w.b) * a.Q + mine.query) * (a.K * a.G) + mine.head) * a.D;
 #pragma unroll
   for (int c = 0; c < NB; ++c)
 #pragma unroll
@@ -804,29 +868,37 @@ __global__ __launch_bounds__(kThreads) void attention_grad_q_kernel(const Args a
       const int d = 32 * c + 8 * g + 4 * (lane / 32);
       const float v[4] = {acc[c][4 * g], acc[c][4 * g + 1], acc[c][4 * g + 2], acc[c][4 * g + 3]};
       if (a.splits > 1)
-        store_four(a.part + split * elements + out_at + d, v, a.D - d, a.D % 4 == 0);
+        store_four(a.part + w.split * elements + out_at + d, v, a.D - d, a.D % 4 == 0);
       else
         store_four(static_cast<T*>(a.grad_q) + out_at + d, v, a.D - d, a.out_vector);
     }
 }
 
 // ---------------------------------------------------------------------------
-// Backward, states: a workgroup's 4 waves hold 32 keys each and walk over the rows (all of the
-// group's heads), so that dk and dv of a key are summed by one wave. Row splits leave fp32
-// sums, which sum_kernel adds in their order.
+// Backward, states: a workgroup's 4 waves hold 32 keys each and walk over the queries of each
+// head of the group in turn, so that dk and dv of a key are summed by one wave. Row splits
+// leave fp32 sums, which sum_kernel adds in their order.
 
 template <typename T, int DP> struct StatesShape {
   static constexpr int kKeys = 32 * kWaves;
   static constexpr int RB = DP * int(sizeof(T)) <= 192 ? 2 : 1;  // blocks of 32 rows in a tile
   static constexpr int kRows = 32 * RB;
   static constexpr int kTile = kRows * Tile<T, DP>::kRowBytes;
-  static constexpr int kBuffers = 2;
-  static constexpr int kRowData = kRows * (3 * 4 + 8);
-  static constexpr int kLds = kBuffers * (2 * kTile + kRowData);
+  static constexpr int kWords = kRows * kWaves * 4;  // a bool mask: 32 keys' bits for each row and wave
+  static constexpr int kBuffer = 2 * kTile + kWords + kRows * 3 * 4;
+  static constexpr int kLds = 2 * kBuffer;
 };
 
+// The non-zero bytes of four as four bits.
+__device__ inline uint32_t byte_bits(uint32_t four) {
+  uint32_t x = four | (four >> 4);
+  x |= x >> 2;
+  x |= x >> 1;
+  return (((x & 0x01010101u) * 0x01020408u) >> 24) & 15u;
+}
+
 template <typename T, int DP, int MASK>
-__global__ __launch_bounds__(kThreads) void attention_grad_states_kernel(const Args a) {
+__global__ __launch_bounds__(kThreads, (kGradStatesWaves<T, DP>)) void attention_grad_states_kernel(const Args a) {
   using Shape = StatesShape<T, DP>;
   using TileT = Tile<T, DP>;
   constexpr int NB = DP / 32, kSteps = TileT::kPieces / 2, kRows = Shape::kRows;
@@ -842,99 +914,145 @@ __global__ __launch_bounds__(kThreads) void attention_grad_states_kernel(const A
   const int bk = int(id / uint32_t(a.row_splits));
   const int b = bk / a.K, kv = bk % a.K;
 
-  const int states = states_of(a, b);
+  const int states = __builtin_amdgcn_readfirstlane(states_of(a, b));
   const int key = key_tile * Shape::kKeys + 32 * wave + lane % 32;
+  const bool words = MASK == kBoolMask && !a.mask_of_keys;
   bool on = key < states;
   if constexpr (MASK == kBoolMask)
     if (a.mask_of_keys && on) on = bool_mask(a, b * a.mask_batch + int64_t(key) * a.mask_key);
 
+  // Tiles of every head of the group in turn.
+  const int query_tiles = (a.Q + kRows - 1) / kRows;
+  const int64_t tiles = int64_t(query_tiles) * a.G;
+  int64_t first = tiles * split / a.row_splits, last = tiles * (split + 1) / a.row_splits;
+  if (key_tile * Shape::kKeys >= states) last = first;  // padding only: zeros
+  int next_head = int(first / (query_tiles ? query_tiles : 1)), next_tile = int(first - int64_t(next_head) * query_tiles);
+
+  Stage<T, DP, kRows> q_stage, go_stage;
+  q_stage.plan(a.q.row, a.Dp);
+  go_stage.plan(a.go.row, a.Dp);
+  float2 stat = {INFINITY, 0.0f};
+  float delta = 0.0f;
+  uint32_t raw[8];
+  int64_t float_at = 0, float_next = 0;  // the tile's first mask element, and its rows (float masks)
+  int float_rows = 0, float_left = 0;
+  auto load = [&]() __attribute__((always_inline)) {  // the next tile
+    const int head = kv * a.G + next_head, query = next_tile * kRows, left = a.Q - query;
+    q_stage.load(static_cast<const T*>(a.q.at) + b * a.q.batch + head * a.q.head + int64_t(query) * a.q.row, left, All());
+    go_stage.load(static_cast<const T*>(a.go.at) + b * a.go.batch + head * a.go.head + int64_t(query) * a.go.row, left,
+                  All());
+    if (threadIdx.x < kRows) {
+      const bool live = int(threadIdx.x) < left;
+      const int64_t at = (int64_t(b) * (a.K * a.G) + head) * a.Q + query + threadIdx.x;
+      stat = live ? a.row_stats[at] : float2{INFINITY, 0.0f};
+      delta = live ? a.delta[at] : 0.0f;
+    }
+    if constexpr (MASK == kFloatMask) {
+      float_next = mask_row_at(a, b, RowOf{query, head});
+      float_left = left;
+    }
+    if (words && threadIdx.x < kRows * kWaves) {  // row threadIdx.x / 4, keys 32 (threadIdx.x % 4) ..
+      const int row = threadIdx.x / kWaves, k0 = key_tile * Shape::kKeys + 32 * int(threadIdx.x % kWaves);
+      const int64_t at = mask_row_at(a, b, RowOf{query + (row < left ? row : left - 1), head});
+      const uint8_t* bytes = static_cast<const uint8_t*>(a.mask) + at;
+      if (a.mask_words && k0 + 32 <= states) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const u32x4 four = *reinterpret_cast<const u32x4*>(bytes + k0 + 16 * i);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) raw[4 * i + j] = four[j];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int k1 = k0 + 4 * i;
+          raw[i] = 0;
+          if (a.mask_quads && k1 + 4 <= states) {
+            raw[i] = *reinterpret_cast<const uint32_t*>(bytes + k1);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (k1 + j < states) raw[i] |= uint32_t(bytes[int64_t(k1 + j) * a.mask_key] != 0) << (8 * j);
+          }
+        }
+      }
+    }
+    if (++next_tile == query_tiles) {
+      next_tile = 0;
+      ++next_head;
+    }
+  };
+  if (first < last) load();
+
   u32x4 k[kSteps], v[kSteps];
   {
-    const T* k_row = static_cast<const T*>(a.k) + b * a.k_batch + int64_t(key) * a.k_row + kv * a.k_head;
-    const T* v_row = static_cast<const T*>(a.v) + b * a.v_batch + int64_t(key) * a.v_row + kv * a.v_head;
+    const T* k_row = static_cast<const T*>(a.k.at) + b * a.k.batch + int64_t(key) * a.k.row + kv * a.k.head;
+    const T* v_row = static_cast<const T*>(a.v.at) + b * a.v.batch + int64_t(key) * a.v.row + kv * a.v.head;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const int c = (2 * s + lane / 32) * N;
       const u32x4 zero = {0, 0, 0, 0};
-      k[s] = on ? load_piece(k_row, c, a.D, a.vector) : zero;
-      v[s] = on ? load_piece(v_row, c, a.D, a.vector) : zero;
+      k[s] = on ? load_piece(k_row, c, a.Dp) : zero;
+      v[s] = on ? load_piece(v_row, c, a.Dp) : zero;
     }
   }
-
-  const int tiles = int((a.R + kRows - 1) / kRows);
-  int first = int(int64_t(tiles) * split / a.row_splits), last = int(int64_t(tiles) * (split + 1) / a.row_splits);
-  if (key_tile * Shape::kKeys >= states) last = first;  // padding only: zeros
-  const T* q_base = static_cast<const T*>(a.q) + b * a.q_batch;
-  const T* go_base = static_cast<const T*>(a.grad_out) + int64_t(b) * a.Q * a.K * a.G * a.D;
-  Stage<T, DP, kRows, kThreads> q_stage, go_stage;
-  float2 stat = {INFINITY, 0.0f};
-  float delta = 0.0f;
-  int64_t mask_at = 0;
-  auto load = [&](int tile) {
-    q_stage.load([&](int row) -> const T* {
-      const uint32_t r = uint32_t(tile) * kRows + row;
-      if (r >= a.R) return nullptr;
-      const RowOf o = row_of(a, kv, r);
-      return q_base + int64_t(o.query) * a.q_row + o.head * a.q_head;
-    }, a.D, a.vector);
-    go_stage.load([&](int row) -> const T* {
-      const uint32_t r = uint32_t(tile) * kRows + row;
-      if (r >= a.R) return nullptr;
-      const RowOf o = row_of(a, kv, r);
-      return go_base + (int64_t(o.query) * (a.K * a.G) + o.head) * a.D;
-    }, a.D, a.out_vector);
-    if (threadIdx.x < kRows) {
-      const uint32_t r = uint32_t(tile) * kRows + threadIdx.x;
-      const bool live = r < a.R;
-      stat = live ? a.row_stats[int64_t(bk) * a.R + r] : float2{INFINITY, 0.0f};
-      delta = live ? a.delta[int64_t(bk) * a.R + r] : 0.0f;
-      if constexpr (MASK != kNoMask) mask_at = mask_row_at(a, b, row_of(a, kv, live ? r : a.R - 1));
-    }
-  };
 
   f32x16 grad_k[NB] = {}, grad_v[NB] = {};
   Scaled<T> scaled;
   const float factor = MASK == kFloatMask ? a.scale : a.scale * kLog2e;
-  if (first < last) load(first);
-  for (int tile = first; tile < last; ++tile) {
-    char* q_tile = lds + ((tile - first) % Shape::kBuffers) * (2 * Shape::kTile + Shape::kRowData);
+  auto step = [&](int64_t tile, auto buffer) __attribute__((always_inline)) {
+    char* q_tile = lds + decltype(buffer)::value * Shape::kBuffer;
     char* go_tile = q_tile + Shape::kTile;
-    int64_t* row_mask = reinterpret_cast<int64_t*>(go_tile + Shape::kTile);
-    float* row_shift = reinterpret_cast<float*>(row_mask + kRows);
-    float* row_delta = row_shift + kRows;
-    float* row_max = row_delta + kRows;  // float masks only
+    uint32_t* row_words = reinterpret_cast<uint32_t*>(go_tile + Shape::kTile);
+    float* row_shift = reinterpret_cast<float*>(row_words + Shape::kWords / 4);
+    float* row_delta = row_shift + kRows;  // minus delta
+    float* row_max = row_delta + kRows;    // float masks only
     q_stage.store(q_tile);
     go_stage.store(go_tile);
     if (threadIdx.x < kRows) {
       row_shift[threadIdx.x] = kWeightBits<T> - (MASK == kFloatMask ? stat.y : stat.x + stat.y);
-      row_delta[threadIdx.x] = delta;
+      row_delta[threadIdx.x] = -delta;
       if constexpr (MASK == kFloatMask) row_max[threadIdx.x] = stat.x;
-      if constexpr (MASK != kNoMask) row_mask[threadIdx.x] = mask_at;
     }
+    if (words && threadIdx.x < kRows * kWaves) {
+      uint32_t word = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) word |= byte_bits(raw[i]) << (4 * i);
+      row_words[(threadIdx.x % kWaves) * kRows + threadIdx.x / kWaves] = word;
+    }
+    float_at = float_next;
+    float_rows = float_left;
     __syncthreads();
-    if (tile + 1 < last) load(tile + 1);
+    if (tile + 1 < last) load();
 
 #pragma unroll
     for (int n = 0; n < Shape::RB; ++n) {
       const int local = 32 * n;
       float add[16];
-      uint32_t bits = on ? 0xffff : 0;
-      if constexpr (MASK == kBoolMask) {
-        if (on) {
-          bits = 0;
+      uint32_t bits = 0xffff;
+      if (words) {
+        bits = 0;
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            bits |= uint32_t(bool_mask(a, row_mask[local + result_row(i)] + int64_t(key) * a.mask_key)) << i;
+        for (int g = 0; g < 4; ++g) {
+          const u32x4 four = *reinterpret_cast<const u32x4*>(row_words + wave * kRows + local + result_row(4 * g));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) bits |= ((four[j] >> (lane % 32)) & 1) << (4 * g + j);
         }
-        if (!__any(bits != 0)) continue;
+        if (!__any(on && bits != 0)) continue;
       } else if constexpr (MASK == kFloatMask) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          add[i] = on ? float_mask(a, row_mask[local + result_row(i)] + int64_t(key) * a.mask_key) : kLowest;
-          if (add[i] == kLowest) bits &= ~(1u << i);
+          const int row = local + result_row(i);
+          add[i] = on && row < float_rows ? float_mask(a, float_at + row * a.mask_row + int64_t(key) * a.mask_key) : kLowest;
         }
       }
-      f32x16 s = {}, dp = {};
+      f32x16 s = {}, dp;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 low = *reinterpret_cast<const f32x4*>(row_delta + local + result_row(4 * g));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dp[4 * g + j] = low[j];
+      }
 #pragma unroll
       for (int t = 0; t < kSteps; ++t) {
         s = Mma<T>::rows(row_piece<T, DP>(q_tile, local, t), k[t], s);
@@ -945,7 +1063,6 @@ __global__ __launch_bounds__(kThreads) void attention_grad_states_kernel(const A
       for (int g = 0; g < 4; ++g) {
         const int at = local + result_row(4 * g);
         const f32x4 shift = *reinterpret_cast<const f32x4*>(row_shift + at);
-        const f32x4 dl = *reinterpret_cast<const f32x4*>(row_delta + at);
         f32x4 top = {};
         if constexpr (MASK == kFloatMask) top = *reinterpret_cast<const f32x4*>(row_max + at);
 #pragma unroll
@@ -953,9 +1070,13 @@ __global__ __launch_bounds__(kThreads) void attention_grad_states_kernel(const A
           const int i = 4 * g + j;
           const float y = MASK == kFloatMask ? fmaf(fmaf(s[i], factor, add[i]) - top[j], kLog2e, shift[j])
                                              : fmaf(s[i], factor, shift[j]);
-          const bool here = (bits >> i) & 1;
-          p[i] = here ? __builtin_amdgcn_exp2f(y) : 0.0f;
-          ds[i] = here ? p[i] * (dp[i] - dl[j]) : 0.0f;
+          p[i] = __builtin_amdgcn_exp2f(y);
+          // Without a mask every state of the tile is attended; columns past the last are
+          // not written.
+          if constexpr (MASK == kBoolMask) p[i] = (bits >> i) & 1 ? p[i] : 0.0f;
+          if constexpr (MASK == kFloatMask) p[i] = add[i] == kLowest ? 0.0f : p[i];
+          ds[i] = p[i] * scaled.power * dp[i];
+          if constexpr (MASK != kNoMask) ds[i] = p[i] == 0.0f ? 0.0f : ds[i];
         }
       }
       const auto wp = Mma<T>::weights(p);
@@ -966,10 +1087,14 @@ __global__ __launch_bounds__(kThreads) void attention_grad_states_kernel(const A
 #pragma unroll
       for (int c = 0; c < NB; ++c) grad_k[c] = accumulate<T, DP>(q_tile, local, c, ws, grad_k[c]);
     }
+  };
+  for (int64_t tile = first; tile < last; tile += 2) {
+    step(tile, Const<0>());
+    if (tile + 1 < last) step(tile + 1, Const<1>());
   }
 
   if (key >= a.S) return;
-  const float unit = __builtin_amdgcn_exp2f(-kWeightBits<T>);
+  const float unit = __builtin_amdgcn_exp2f(-kWeightBits<T>), undo = scaled.undo();
   const int64_t at = ((int64_t(b) * a.S + key) * a.K + kv) * a.D;
   const int64_t elements = int64_t(a.B) * a.S * a.K * a.D;
 #pragma unroll
@@ -980,8 +1105,8 @@ __global__ __launch_bounds__(kThreads) void attention_grad_states_kernel(const A
       float x[4], y[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        x[i] = scaled.undo(grad_k[c][4 * g + i]) * (unit * a.scale);
-        y[i] = grad_v[c][4 * g + i] * unit;
+        x[i] = on ? grad_k[c][4 * g + i] * undo * (unit * a.scale) : 0.0f;
+        y[i] = on ? grad_v[c][4 * g + i] * unit : 0.0f;
       }
       if (a.row_splits > 1) {
         store_four(a.part_k + split * elements + at + d, x, a.D - d, a.D % 4 == 0);
@@ -1005,6 +1130,7 @@ __global__ __launch_bounds__(256) void attention_sum_kernel(const float* part, i
   }
   float v[4] = {};
   const bool vector = n % 4 == 0;
+#pragma unroll 4
   for (int s = 0; s < count; ++s) {
     const float* p = part + s * n + at;
     if (vector) {
@@ -1020,11 +1146,30 @@ __global__ __launch_bounds__(256) void attention_sum_kernel(const float* part, i
   store_four(out + at, v, int(n - at < 4 ? n - at : 4), vector && reinterpret_cast<uintptr_t>(out) % 16 == 0);
 }
 
+// Rows of D channels at any strides and alignment, as dense rows of Dp with zeros past D: one
+// thread per 16 bytes of the copy.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_pack_kernel(Rows from, T* to, int64_t rows, int heads, int D, int Dp,
+                                                             int64_t pieces) {
+  constexpr int N = 16 / int(sizeof(T));
+  const int64_t n = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (n >= pieces) return;
+  const int each = Dp / N, d = int(n % each) * N;
+  int64_t at = n / each;
+  const int64_t head = at % heads;
+  at /= heads;
+  const T* row = static_cast<const T*>(from.at) + (at / rows) * from.batch + (at % rows) * from.row + head * from.head;
+  T parts[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) parts[i] = d + i < D ? row[d + i] : T(0);
+  u32x4 out;
+  __builtin_memcpy(&out, parts, 16);
+  *reinterpret_cast<u32x4*>(to + n * N) = out;
+}
+
 // ---------------------------------------------------------------------------
 // Launches, one translation unit for each type (attention_f32.hip and so on): the kernels'
 // variants compile side by side.
-
-template <int V> using Const = std::integral_constant<int, V>;
 
 template <typename F> void with_mask(int kind, F f) {
   if (kind == kNoMask) f(Const<kNoMask>());
@@ -1047,6 +1192,8 @@ template <typename F> void with_channels(int64_t D, F f) {
 template <typename T> void launch_forward(const Args& a, int mask_kind, bool few_rows, uint32_t groups, hipStream_t s);
 template <typename T>
 void launch_backward(const Args& a, int mask_kind, bool few_rows, uint32_t groups, uint32_t key_groups, hipStream_t s);
+template <typename T>
+void launch_pack(const Rows& from, void* to, int64_t batch, int64_t rows, int heads, int D, int Dp, hipStream_t s);
 
 #ifdef ATTENTION_DEFINE_LAUNCHES
 
@@ -1060,8 +1207,10 @@ template <typename T> void launch_forward(const Args& a, int mask_kind, bool few
     });
   });
   if (a.splits > 1) {
-    const int64_t threads = int64_t(a.B) * a.K * a.R * ((a.D + 3) / 4);
-    attention_combine_kernel<T><<<uint32_t(ceil_div(threads, 256)), 256, 0, s>>>(a, mask_kind == kFloatMask);
+    int lanes = 1;
+    while (4 * lanes < a.D) lanes *= 2;
+    attention_combine_kernel<T><<<uint32_t(ceil_div(int64_t(a.B) * a.K * a.R, kWaves)), kThreads, 0, s>>>(
+        a, lanes, mask_kind == kFloatMask);
   }
 }
 
@@ -1092,10 +1241,18 @@ void launch_backward(const Args& a, int mask_kind, bool few_rows, uint32_t group
   }
 }
 
+template <typename T>
+void launch_pack(const Rows& from, void* to, int64_t batch, int64_t rows, int heads, int D, int Dp, hipStream_t s) {
+  const int64_t pieces = batch * rows * heads * (Dp / (16 / int64_t(sizeof(T))));
+  if (pieces == 0) return;
+  attention_pack_kernel<T><<<uint32_t(ceil_div(pieces, 256)), 256, 0, s>>>(from, static_cast<T*>(to), rows, heads, D, Dp, pieces);
+}
+
 #define ATTENTION_INSTANTIATE(T)                                                                        \
   namespace attention {                                                                                 \
   template void launch_forward<T>(const Args&, int, bool, uint32_t, hipStream_t);                       \
   template void launch_backward<T>(const Args&, int, bool, uint32_t, uint32_t, hipStream_t);            \
+  template void launch_pack<T>(const Rows&, void*, int64_t, int64_t, int, int, int, hipStream_t);       \
   }
 
 #endif

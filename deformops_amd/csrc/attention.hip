@@ -11,37 +11,71 @@ constexpr int kWanted = 512;  // workgroups that fill 256 CUs twice
 
 int element_size(int dtype) { return dtype == MSDA_F32 ? 4 : dtype == MSDA_F16 || dtype == MSDA_BF16 ? 2 : 0; }
 
+int64_t round_up(int64_t n) { return (n + 255) / 256 * 256; }
+
+// Whether the kernels read these rows as they are: 16-byte pieces, and steps from row to row
+// that a tile's 32-bit offsets hold and that tell the rows apart.
+bool rows_as_they_are(const deformops_attention& c, const void* p, const int64_t (&strides)[3], int64_t rows) {
+  const int size = element_size(c.dtype), n = 16 / size;
+  return c.channels % n == 0 && aligned(p, 16) && strides[0] % n == 0 && strides[1] % n == 0 && strides[2] % n == 0 &&
+         (rows <= 1 || (strides[1] >= c.channels && strides[1] * size <= (int64_t(1) << 23)));
+}
+
+// Where one operand's packed copy lies in the workspace, if it has one.
+struct Packed {
+  bool on;
+  int64_t at;
+};
+
 struct Plan {
   bool few_rows;   // one row tile of 32: the waves share the rows
   int splits;      // of the keys
   int row_splits;  // of the rows, in the states' kernel
   int64_t forward_bytes, backward_bytes;
   int64_t delta_at, part_at, part_stats_at, part_k_at, part_v_at;
+  Packed q, k, v, o, go;
 };
 
-int64_t round_up(int64_t n) { return (n + 255) / 256 * 256; }
-
+// `grad_output` and the output are dense: one packing rule for both by alignment (the size
+// query assumes aligned ones, the launch checks).
 Plan plan_of(const deformops_attention& c) {
   Plan p = {};
   const int64_t G = c.heads / c.key_heads, R = c.queries * G, BK = c.batch * c.key_heads;
-  const int DP = padded(c.channels), size = element_size(c.dtype);
+  const int DP = padded(c.channels), size = element_size(c.dtype), n = 16 / size;
   p.few_rows = R <= 64 && size * DP < 512;
   const int64_t rows = p.few_rows ? 32 : 128, keys = p.few_rows ? 128 : 64;
   const int64_t groups = BK * ceil_div(R, rows), tiles = ceil_div(c.keys, keys);
   p.splits = int(std::max<int64_t>(1, std::min<int64_t>(ceil_div(kWanted, std::max<int64_t>(1, groups)), tiles / 2)));
   const int64_t row_tile = DP * size <= 192 ? 64 : 32;
-  const int64_t key_groups = BK * ceil_div(c.keys, 128), row_tiles = ceil_div(R, row_tile);
+  const int64_t key_groups = BK * ceil_div(c.keys, 128), row_tiles = G * ceil_div(c.queries, row_tile);
   p.row_splits = int(std::max<int64_t>(1, std::min<int64_t>(ceil_div(kWanted, std::max<int64_t>(1, key_groups)), row_tiles / 2)));
 
-  const int64_t part = p.splits > 1 ? round_up(p.splits * BK * R * c.channels * 4) : 0;
-  p.part_at = 0;
-  p.part_stats_at = part;
-  p.forward_bytes = part + (p.splits > 1 ? round_up(p.splits * BK * R * 8) : 0);
-  p.delta_at = part;
-  const int64_t states = p.row_splits > 1 ? round_up(p.row_splits * c.batch * c.keys * c.key_heads * c.channels * 4) : 0;
-  p.part_k_at = part + round_up(BK * R * 4);
-  p.part_v_at = p.part_k_at + states;
-  p.backward_bytes = p.part_v_at + states;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += round_up(bytes);
+    return here;
+  };
+  const int64_t Dp = ceil_div(c.channels, n) * n;
+  auto pack = [&](bool as_it_is, int64_t rows_of, int64_t heads) {
+    return as_it_is ? Packed{false, 0} : Packed{true, take(c.batch * rows_of * heads * Dp * size)};
+  };
+  p.q = pack(rows_as_they_are(c, c.query, c.query_strides, c.queries), c.queries, c.heads);
+  p.k = pack(rows_as_they_are(c, c.key, c.key_strides, c.keys), c.keys, c.key_heads);
+  p.v = pack(rows_as_they_are(c, c.value, c.value_strides, c.keys), c.keys, c.key_heads);
+  p.part_at = take(p.splits > 1 ? p.splits * BK * R * c.channels * 4 : 0);
+  const int64_t shared = at;
+  p.part_stats_at = take(p.splits > 1 ? p.splits * BK * R * 8 : 0);
+  p.forward_bytes = at;
+  at = shared;
+  const bool dense = c.channels % n == 0;
+  p.o = pack(dense, c.queries, c.heads);
+  p.go = pack(dense, c.queries, c.heads);
+  p.delta_at = take(BK * R * 4);
+  const int64_t states = p.row_splits > 1 ? p.row_splits * c.batch * c.keys * c.key_heads * c.channels * 4 : 0;
+  p.part_k_at = take(states);
+  p.part_v_at = take(states);
+  p.backward_bytes = at;
   return p;
 }
 
@@ -70,25 +104,40 @@ int check(const deformops_attention* c) {
   return MSDA_OK;
 }
 
-bool rows_aligned(const deformops_attention& c, const void* p, const int64_t (&strides)[3]) {
-  const int n = 16 / element_size(c.dtype);
-  return aligned(p, 16) && strides[0] % n == 0 && strides[1] % n == 0 && strides[2] % n == 0;
+template <typename F> void with_type(int dtype, F f);
+
+// An operand's rows as the kernels read them, packed by a launch where they have to be.
+Rows rows_of(const deformops_attention& c, const void* p, const int64_t (&strides)[3], Packed packed, int64_t rows,
+             int64_t heads, char* workspace, hipStream_t s) {
+  // The step past a single row may be anything; it bounds the tile's range of bytes.
+  const Rows from = {p, strides[0], rows > 1 ? strides[1] : c.channels, strides[2]};
+  if (!packed.on) return from;
+  const int64_t n = 16 / element_size(c.dtype), Dp = ceil_div(c.channels, n) * n;
+  void* to = workspace + packed.at;
+  with_type(c.dtype, [&](auto t) {
+    launch_pack<decltype(t)>(from, to, c.batch, rows, int(heads), int(c.channels), int(Dp), s);
+  });
+  return Rows{to, rows * heads * Dp, heads * Dp, Dp};
 }
 
-Args args_of(const deformops_attention& c, const Plan& p, void* workspace) {
+Args args_of(const deformops_attention& c, const Plan& p, void* workspace, hipStream_t s) {
   Args a = {};
-  a.q = c.query; a.k = c.key; a.v = c.value;
-  a.q_batch = c.query_strides[0]; a.q_row = c.query_strides[1]; a.q_head = c.query_strides[2];
-  a.k_batch = c.key_strides[0]; a.k_row = c.key_strides[1]; a.k_head = c.key_strides[2];
-  a.v_batch = c.value_strides[0]; a.v_row = c.value_strides[1]; a.v_head = c.value_strides[2];
+  char* ws = static_cast<char*>(workspace);
+  a.q = rows_of(c, c.query, c.query_strides, p.q, c.queries, c.heads, ws, s);
+  a.k = rows_of(c, c.key, c.key_strides, p.k, c.keys, c.key_heads, ws, s);
+  a.v = rows_of(c, c.value, c.value_strides, p.v, c.keys, c.key_heads, ws, s);
   if (c.mask_kind != kNoMask) {
     const int size = c.mask_kind == kBoolMask ? 1 : element_size(c.mask_dtype);
     a.mask = c.mask;
     a.mask_batch = c.mask_strides[0]; a.mask_head = c.mask_strides[1];
     a.mask_row = c.mask_strides[2]; a.mask_key = c.mask_strides[3];
     a.mask_type = c.mask_dtype;
-    a.mask_quads = c.mask_strides[3] == 1 && aligned(c.mask, 4 * size) && c.mask_strides[0] % 4 == 0 &&
-                   c.mask_strides[1] % 4 == 0 && c.mask_strides[2] % 4 == 0;
+    auto together = [&](int64_t n) {
+      return c.mask_strides[3] == 1 && aligned(c.mask, size_t(n) * size) && c.mask_strides[0] % n == 0 &&
+             c.mask_strides[1] % n == 0 && c.mask_strides[2] % n == 0;
+    };
+    a.mask_quads = together(4);
+    a.mask_words = together(16);
     a.mask_of_keys = c.mask_kind == kBoolMask && (c.mask_strides[1] == 0 || c.heads == 1) &&
                      (c.mask_strides[2] == 0 || c.queries == 1);
   }
@@ -97,14 +146,12 @@ Args args_of(const deformops_attention& c, const Plan& p, void* workspace) {
   a.out = c.output;
   a.B = int(c.batch); a.Q = int(c.queries); a.S = int(c.keys); a.K = int(c.key_heads);
   a.G = int(c.heads / c.key_heads); a.D = int(c.channels);
+  const int n = 16 / element_size(c.dtype);
+  a.Dp = int(ceil_div(a.D, n) * n);
   a.R = uint32_t(c.queries * a.G);
   a.scale = c.scale;
-  const int n = 16 / element_size(c.dtype);
-  a.vector = a.D % n == 0 && rows_aligned(c, c.query, c.query_strides) && rows_aligned(c, c.key, c.key_strides) &&
-             rows_aligned(c, c.value, c.value_strides);
   a.splits = p.splits;
   a.row_splits = p.row_splits;
-  char* ws = static_cast<char*>(workspace);
   a.part = reinterpret_cast<float*>(ws + p.part_at);
   a.part_stats = reinterpret_cast<float2*>(ws + p.part_stats_at);
   a.delta = reinterpret_cast<float*>(ws + p.delta_at);
@@ -150,13 +197,13 @@ int deformops_cross_attention_forward(const deformops_attention* c, void* row_st
   if (p.forward_bytes && (!workspace || workspace_bytes < p.forward_bytes || !aligned(workspace, 256)))
     return fail(MSDA_ERR_INVALID, "cross attention: the workspace must hold %lld bytes, aligned to 256",
                 static_cast<long long>(p.forward_bytes));
-  Args a = args_of(*c, p, workspace);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  Args a = args_of(*c, p, workspace, s);
   a.stats = static_cast<float2*>(row_stats);
   a.out_vector = a.D % 4 == 0 && aligned(c->output, 16);
   const int64_t rows = p.few_rows ? 32 : 128;
   const int64_t groups = int64_t(a.B) * a.K * ceil_div(a.R, rows) * a.splits;
   if (const int e = too_many(groups)) return e;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
   with_type(c->dtype, [&](auto t) { launch_forward<decltype(t)>(a, c->mask_kind, p.few_rows, uint32_t(groups), s); });
   return launched("cross attention forward");
 }
@@ -174,20 +221,23 @@ int deformops_cross_attention_backward(const deformops_attention* c, const void*
   if (p.backward_bytes && (!workspace || workspace_bytes < p.backward_bytes || !aligned(workspace, 256)))
     return fail(MSDA_ERR_INVALID, "cross attention: the workspace must hold %lld bytes, aligned to 256",
                 static_cast<long long>(p.backward_bytes));
-  Args a = args_of(*c, p, workspace);
+  const int n = 16 / element_size(c->dtype);
+  if (!aligned(c->output, 16) || !aligned(grad_output, 16))
+    return fail(MSDA_ERR_INVALID, "cross attention: output and grad_output must be aligned to 16 bytes");
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  Args a = args_of(*c, p, workspace, s);
+  const int64_t dense[3] = {c->queries * c->heads * c->channels, c->heads * c->channels, c->channels};
+  a.o = rows_of(*c, c->output, dense, p.o, c->queries, c->heads, static_cast<char*>(workspace), s);
+  a.go = rows_of(*c, grad_output, dense, p.go, c->queries, c->heads, static_cast<char*>(workspace), s);
   a.row_stats = static_cast<const float2*>(row_stats);
-  a.grad_out = grad_output;
   a.grad_q = grad_query;
   a.grad_k = grad_key;
   a.grad_v = grad_value;
-  const int n = 16 / element_size(c->dtype);
-  a.out_vector = a.D % n == 0 && aligned(c->output, 16) && aligned(grad_output, 16) && aligned(grad_query, 16) &&
-                 aligned(grad_key, 16) && aligned(grad_value, 16);
+  a.out_vector = a.D % n == 0 && aligned(grad_query, 16) && aligned(grad_key, 16) && aligned(grad_value, 16);
   const int64_t rows = p.few_rows ? 32 : 128;
   const int64_t groups = int64_t(a.B) * a.K * ceil_div(a.R, rows) * a.splits;
   const int64_t key_groups = int64_t(a.B) * a.K * ceil_div(a.S, 128) * a.row_splits;
   if (const int e = too_many(std::max(groups, key_groups))) return e;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
   with_type(c->dtype, [&](auto t) {
     launch_backward<decltype(t)>(a, c->mask_kind, p.few_rows, uint32_t(groups), uint32_t(key_groups), s);
   });

@@ -325,17 +325,18 @@ typedef struct deformops_attention {
 } deformops_attention;
 
 /* Bytes of workspace the forward and the backward of such a call take (0: none); reads
- * the sizes and types only. Host only. */
+ * sizes, types, strides and the alignment of the operands (rows that are not made of
+ * aligned 16-byte pieces are packed into it first). Host only. */
 int deformops_cross_attention_workspace_size(const deformops_attention* call, int64_t* forward,
                                              int64_t* backward);
 
-/* Writes output and, unless row_stats is null, two floats for each (image, key head, query,
- * head of the group), for the backward. The workspace is aligned to 256 bytes. */
+/* Writes output and, unless row_stats is null, two floats for each (image, head, query), for
+ * the backward. The workspace is aligned to 256 bytes. */
 int deformops_cross_attention_forward(const deformops_attention* call, void* row_stats,
                                       void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Writes the three gradients, dense in the layouts above, from the forward's output and
- * row_stats and the dense grad_output. Sums are in fp32 and in an order that the sizes
+ * row_stats and the dense grad_output (both aligned to 16 bytes). Sums are in fp32 and in an order that the sizes
  * fix: equal calls give equal bits. The mask has no gradient. */
 int deformops_cross_attention_backward(const deformops_attention* call, const void* row_stats,
                                        const void* grad_output, void* grad_query, void* grad_key,

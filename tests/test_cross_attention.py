@@ -11,8 +11,9 @@ Tolerances. With u half a step of the dtype (eps / 2), e = 2^-24, and s the scal
 - ds is rounded once more (u |ds|), and every result once (u |result|);
 - below the normal numbers a rounding is off by half a smallest step instead of u: v_exp_f32
   gives 0 below 2^-126, so a float32 weight is off by up to 2^-126 more; a float16 operand
-  holds weights times 2^14, whose smallest step 2^-24 is 2^-38 of a weight: off by 2^-39
-  more; and ds times a power of two that puts the largest of its row (in dq) or key (in dk)
+  holds exp(x - m) times 2^9 in the forward (times 2^14 in the backward), m at most the
+  row's maximum, whose smallest step 2^-24 is 2^-33 (2^-38): off by 2^-34 (2^-39) more of
+  a sum that is at least 1; and ds times a power of two that puts the largest of its row (in dq) or key (in dk)
   above 2^11: off by 2^-25 / 2^11 = 2^-36 of that more.
 
 The bounds below add these up, element by element, in 64 bits.
@@ -74,7 +75,7 @@ def reference(q, k, v, mask=None, lengths=None, scale=None, grad=None):
     p = torch.softmax(s, -1).nan_to_num(nan=0.0) if S else s
     attended = (~off).double()
     w_err = p * (2 * e_s + (S + 8) * e) + 2.0**-126 * attended  # of a weight in float32
-    p_err = w_err + weights_u * p + (2.0**-39 * attended if q_type == F16 else 0.0)
+    p_err = w_err + weights_u * p + (2.0**-34 * attended if q_type == F16 else 0.0)
     o = p @ v4
     o_err = p_err @ v4.abs() + S * e * (p @ v4.abs()) + u * o.abs()
 
