@@ -60,9 +60,8 @@ struct Args {
   Rows q, k, v;
   const void* mask;
   int64_t mask_batch, mask_head, mask_row, mask_key;
-  int mask_type;    // element type of a float mask
-  bool mask_quads;  // four keys of a row lie side by side, aligned to their size
-  bool mask_words;  // 16 of them
+  int mask_row_keys;  // keys of a mask's row in memory, side by side (at least 4)
+  int mask_type;      // element type of a float mask
   bool mask_of_keys;  // a bool mask that is one for all rows and heads: it removes states
   const void* lengths;
   bool lengths_i64;
@@ -73,15 +72,18 @@ struct Args {
   uint32_t R;  // rows of one (image, key head): Q * G
   float scale;
   bool out_vector;  // results may be written four channels at a time
-  int splits;
-  float* part;         // [splits][B * K][R][D] unnormalized sums of each split
-  float2* part_stats;  // [splits][B * K][R]
+  // The key axis is worked on in `slots` pieces, which belong to images: `splits` of each, or,
+  // `balanced`, as many of each as its states need.
+  int slots, splits;
+  bool balanced;
+  float* part;         // [slots][K][R][D] unnormalized sums of each piece
+  float2* part_stats;  // [slots][K][R]
   // Backward.
   Rows o, go;
   const float2* row_stats;
   float* delta;  // [B][H][Q]
   void *grad_q, *grad_k, *grad_v;
-  int row_splits;
+  int row_splits, near;
   float* part_k;  // [row_splits][B][S][K][D]
   float* part_v;
 };
@@ -281,45 +283,65 @@ __device__ inline float float_mask(const Args& a, int64_t at) {
 }
 __device__ inline bool bool_mask(const Args& a, int64_t at) { return static_cast<const uint8_t*>(a.mask)[at] != 0; }
 
+// Mask rows may begin at any byte: global loads take any alignment.
+template <typename V> __device__ inline V load_anywhere(const void* p) {
+  struct __attribute__((packed)) Any { V v; };
+  return static_cast<const Any*>(p)->v;
+}
+
+// Four bytes of a mask's row from key k0: keys past the row are 0.
+__device__ inline uint32_t four_bytes(const Args& a, const uint8_t* row, int k0) {
+  const int at = min(k0, a.mask_row_keys - 4), past = k0 - at;
+  const uint32_t four = load_anywhere<uint32_t>(row + at);
+  return past > 3 ? 0 : four >> (8 * past);
+}
+
 // A bool mask's bytes for the 16 result rows (32 keys from `key`) of the row whose first mask
-// element is `at`: four words, result row r in byte r % 4 of word r / 4. Keys at or past `limit`
-// are left out.
+// element is `at`: four words, result row r in byte r % 4 of word r / 4.
 struct MaskBytes {
   uint32_t word[4];
   __device__ bool any() const { return (word[0] | word[1] | word[2] | word[3]) != 0; }
   __device__ bool on(int r) const { return ((word[r / 4] >> (8 * (r % 4))) & 0xff) != 0; }
 };
-__device__ __forceinline__ MaskBytes mask_bytes(const Args& a, int64_t at, int key, int limit) {
-  MaskBytes out = {};
-  const int half = (threadIdx.x % kWave) / 32;
+__device__ __forceinline__ MaskBytes mask_bytes(const Args& a, int64_t at, int key) {
+  MaskBytes out;
+  const uint8_t* row = static_cast<const uint8_t*>(a.mask) + at;
+  const int k0 = key + 4 * (int(threadIdx.x % kWave) / 32);
+  if (key + 32 <= a.mask_row_keys) {
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const int k0 = key + 8 * g + 4 * half;
-    if (a.mask_quads && k0 + 4 <= limit) {
-      out.word[g] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.mask) + at + k0);
-    } else {
+    for (int g = 0; g < 4; ++g) out.word[g] = load_anywhere<uint32_t>(row + k0 + 8 * g);
+  } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (k0 + i < limit) out.word[g] |= uint32_t(bool_mask(a, at + int64_t(k0 + i) * a.mask_key)) << (8 * i);
-    }
+    for (int g = 0; g < 4; ++g) out.word[g] = four_bytes(a, row, k0 + 8 * g);
   }
   return out;
 }
 
-// The additive mask of the 16 result rows, -inf at or past `limit`.
-__device__ __forceinline__ void float_masks(const Args& a, int64_t at, int key, int limit, float (&out)[16]) {
-  const int half = (threadIdx.x % kWave) / 32;
+// The additive mask of the 16 result rows; 0 past the row.
+__device__ __forceinline__ void float_masks(const Args& a, int64_t at, int key, float (&out)[16]) {
+  const int k0 = key + 4 * (int(threadIdx.x % kWave) / 32);
+  if (key + 32 > a.mask_row_keys) {
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const int k0 = key + 8 * g + 4 * half;
-    if (a.mask_quads && k0 + 4 <= limit && a.mask_type == MSDA_F32) {
-      const f32x4 four = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.mask) + at + k0);
+    for (int i = 0; i < 16; ++i) {
+      const int k = k0 + 8 * (i / 4) + i % 4;
+      out[i] = k < a.mask_row_keys ? float_mask(a, at + k) : 0.0f;
+    }
+  } else if (a.mask_type == MSDA_F32) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 four = load_anywhere<f32x4>(static_cast<const float*>(a.mask) + at + k0 + 8 * g);
 #pragma unroll
       for (int i = 0; i < 4; ++i) out[4 * g + i] = four[i];
-    } else {
+    }
+  } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        out[4 * g + i] = k0 + i < limit ? float_mask(a, at + int64_t(k0 + i) * a.mask_key) : kLowest;
+    for (int g = 0; g < 4; ++g) {
+      const u32x2 two = load_anywhere<u32x2>(static_cast<const uint16_t*>(a.mask) + at + k0 + 8 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint16_t h = uint16_t(two[i / 2] >> (16 * (i % 2)));
+        out[4 * g + i] = a.mask_type == MSDA_BF16 ? __uint_as_float(uint32_t(h) << 16) : widen(__builtin_bit_cast(f16_t, h));
+      }
     }
   }
 }
@@ -395,9 +417,12 @@ struct All {
 };
 
 // Two waves of a SIMD hide each other's waits where their registers allow it (256 each).
-template <typename T, int DP> constexpr int kForwardWaves = sizeof(T) == 4 && DP > 64 ? 1 : 2;
-template <typename T, int DP> constexpr int kGradQWaves = DP * int(sizeof(T)) <= (sizeof(T) == 4 ? 128 : 192) ? 2 : 1;
-template <typename T, int DP> constexpr int kGradStatesWaves = DP * int(sizeof(T)) <= 128 ? 2 : 1;
+template <typename T, int DP, int MASK> constexpr int kForwardWaves =
+    sizeof(T) == 4 ? (DP > 64 ? 1 : 2) : DP == 32 ? (MASK ? 3 : 4) : DP == 64 ? (MASK ? 2 : 3) : DP == 128 && MASK ? 1 : 2;
+template <typename T, int DP, int MASK> constexpr int kGradQWaves =
+    sizeof(T) == 4 ? (DP > 32 ? 1 : 2) : DP == 32 ? 3 : DP <= (MASK ? 64 : 96) ? 2 : 1;
+template <typename T, int DP, int MASK> constexpr int kGradStatesWaves =
+    sizeof(T) == 4 ? (DP > 32 ? 1 : 2) : DP == 32 ? (MASK ? 2 : 3) : DP == 64 ? 2 : 1;
 
 // ---------------------------------------------------------------------------
 // Forward. A workgroup has 4 waves: WR of them along the rows (32 each), 4 / WR along the keys
@@ -410,7 +435,7 @@ template <typename T, int DP, int WR> struct ForwardShape {
   static constexpr int kRows = 32 * WR;
   static constexpr int kKeys = 32 * KB * WK;
   static constexpr int kTile = kKeys * Tile<T, DP>::kRowBytes;
-  static constexpr int kBuffers = 4 * kTile <= (kForwardWaves<T, DP> == 2 ? 80 : 128) * 1024 ? 2 : 1;
+  static constexpr int kBuffers = 4 * kTile <= (kForwardWaves<T, DP, kNoMask> > 1 ? 80 : 128) * 1024 ? 2 : 1;
   static constexpr int kJoin = WK > 1 ? WK * 32 * WR * (DP + 2) * 4 : 0;
   static constexpr int kLds = std::max(2 * kBuffers * kTile, kJoin);
 };
@@ -452,25 +477,68 @@ template <int NB> struct Softmax {
   }
 };
 
-// What a workgroup of the walks over the keys works on.
+// The pieces of image `b`, slots first .. first + count - 1, by the whole wave. With lengths that
+// differ, equal pieces for every image would leave most of the card to wait for the longest one:
+// so every piece gets the same number of tiles (at least 2), and an image as many pieces as its
+// states need, none for none. The sum over images of ceil(tiles / quota) is at most
+// (sum of tiles) / quota + B, which the quota keeps within the slots.
+struct Pieces {
+  int first, count;
+};
+struct Shares {
+  int mine, before;  // of the image of this lane's number
+  __device__ Shares(const Args& a, int keys) {
+    const int lane = threadIdx.x % kWave;
+    const int tiles = lane < a.B ? (states_of(a, lane) + keys - 1) / keys : 0;
+    int64_t total = tiles;
+    for (int by = 32; by; by /= 2) total += __shfl_xor(total, by);
+    const int64_t most = a.slots - a.B, quota = max(int64_t(2), (total + most - 1) / most);
+    mine = int((tiles + quota - 1) / quota);
+    int upto = mine;
+    for (int by = 1; by < kWave; by *= 2) {
+      const int other = __shfl_up(upto, by);
+      if (lane >= by) upto += other;
+    }
+    before = upto - mine;
+  }
+};
+__device__ inline Pieces pieces_of(const Args& a, int b, int keys) {
+  if (!a.balanced) return Pieces{b * a.splits, a.splits};
+  const Shares s(a, keys);
+  return Pieces{__builtin_amdgcn_readlane(s.before, b), __builtin_amdgcn_readlane(s.mine, b)};
+}
+
+// What a workgroup of the walks over the keys works on. Row tiles of one piece of one key head
+// come first, then the heads: their rows share cache lines.
 template <typename Shape> struct KeyWalk {
-  int b, kv, bk, split, first, last, states;
+  int b, kv, slot, first, last, states;
   uint32_t row_tile;
+  bool leads;  // the first piece of its image
 
   __device__ explicit KeyWalk(const Args& a) {
     const uint32_t row_tiles = (a.R + Shape::kRows - 1) / Shape::kRows;
     uint32_t id = xcd_order(blockIdx.x, gridDim.x);
     row_tile = id % row_tiles;
     id /= row_tiles;
-    split = int(id % uint32_t(a.splits));
-    bk = int(id / uint32_t(a.splits));
-    b = bk / a.K;
-    kv = bk % a.K;
+    kv = int(id % uint32_t(a.K));
+    slot = int(id / uint32_t(a.K));
+    int split = slot % a.splits, count = a.splits;
+    b = slot / a.splits;
+    if (a.balanced) {
+      const Shares s(a, Shape::kKeys);
+      const uint64_t here = __ballot(s.before <= slot && slot < s.before + s.mine);
+      b = here ? __builtin_ctzll(here) : -1;
+      if (b < 0) return;
+      split = slot - __builtin_amdgcn_readlane(s.before, b);
+      count = __builtin_amdgcn_readlane(s.mine, b);
+    }
+    leads = split == 0;
     states = __builtin_amdgcn_readfirstlane(states_of(a, b));
     const int tiles = (states + Shape::kKeys - 1) / Shape::kKeys;
-    first = int(int64_t(tiles) * split / a.splits);
-    last = int(int64_t(tiles) * (split + 1) / a.splits);
+    first = int(int64_t(tiles) * split / count);
+    last = int(int64_t(tiles) * (split + 1) / count);
   }
+  __device__ int64_t part_row(const Args& a, uint32_t r) const { return (int64_t(slot) * a.K + kv) * a.R + r; }
 };
 
 // The tiles of keys and values on their way to LDS, and a bool mask's bytes of the next tile.
@@ -506,13 +574,13 @@ template <typename T, int DP, int MASK, typename Shape> struct KeyStage {
     }
     if constexpr (MASK == kBoolMask) {
 #pragma unroll
-      for (int n = 0; n < KB; ++n) next[n] = mask_bytes(a, mask_at, key + local + 32 * n, w.states);
+      for (int n = 0; n < KB; ++n) next[n] = mask_bytes(a, mask_at, key + local + 32 * n);
     }
   }
 };
 
 template <typename T, int DP, int MASK, int WR>
-__global__ __launch_bounds__(kThreads, (kForwardWaves<T, DP>)) void attention_forward_kernel(const Args a) {
+__global__ __launch_bounds__(kThreads, (kForwardWaves<T, DP, MASK>)) void attention_forward_kernel(const Args a) {
   using Shape = ForwardShape<T, DP, WR>;
   using TileT = Tile<T, DP>;
   constexpr int KB = Shape::KB, NB = DP / 32, kSteps = TileT::kPieces / 2, kKeys = Shape::kKeys;
@@ -521,6 +589,7 @@ __global__ __launch_bounds__(kThreads, (kForwardWaves<T, DP>)) void attention_fo
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int wr = wave % WR, wk = wave / WR;
   const KeyWalk<Shape> w(a);
+  if (w.b < 0) return;  // a slot that no image needs
   const uint32_t r = w.row_tile * Shape::kRows + 32 * wr + lane % 32;
   const bool live = r < a.R;
   const RowOf mine = row_of(a, w.kv, live ? r : a.R - 1);
@@ -567,7 +636,7 @@ __global__ __launch_bounds__(kThreads, (kForwardWaves<T, DP>)) void attention_fo
 #pragma unroll
     for (int n = 0; n < KB; ++n) {
       float add[16];
-      if constexpr (MASK == kFloatMask) float_masks(a, mask_at, key0 + 32 * n, w.states, add);
+      if constexpr (MASK == kFloatMask) float_masks(a, mask_at, key0 + 32 * n, add);
       f32x16 s = {};
 #pragma unroll
       for (int t = 0; t < kSteps; ++t) s = Mma<T>::rows(row_piece<T, DP>(k_tile, local + 32 * n, t), q[t], s);
@@ -578,7 +647,7 @@ __global__ __launch_bounds__(kThreads, (kForwardWaves<T, DP>)) void attention_fo
         if constexpr (MASK == kFloatMask) x[n][i] = add[i] == kLowest ? kLowest : fmaf(s[i], factor, add[i]);
       }
     }
-    if (MASK == kNoMask && key0 + 32 * KB > w.states) {
+    if (key0 + 32 * KB > w.states) {
 #pragma unroll
       for (int n = 0; n < KB; ++n)
 #pragma unroll
@@ -655,7 +724,7 @@ __global__ __launch_bounds__(kThreads, (kForwardWaves<T, DP>)) void attention_fo
   if (!live) return;
 
   if (a.splits > 1) {
-    const int64_t at = (int64_t(w.split) * a.B * a.K + w.bk) * a.R + r;
+    const int64_t at = w.part_row(a, r);
     if (lane < 32) a.part_stats[at] = float2{soft.m, soft.l};
     float* part = a.part + at * a.D;
 #pragma unroll
@@ -689,23 +758,27 @@ __global__ __launch_bounds__(kThreads, (kForwardWaves<T, DP>)) void attention_fo
 // each, and 64 / lanes of them in a wave share its splits, so that few rows of many splits do
 // not wait for one lane's loads in turn.
 template <typename T>
-__global__ __launch_bounds__(256) void attention_combine_kernel(const Args a, int lanes, bool natural) {
+__global__ __launch_bounds__(256) void attention_combine_kernel(const Args a, int lanes, bool natural, int keys) {
   const int64_t rows = int64_t(a.B) * a.K * a.R;
   const int64_t row = int64_t(blockIdx.x) * kWaves + threadIdx.x / kWave;
   if (row >= rows) return;  // whole waves
   const int lane = threadIdx.x % kWave, share = lane / lanes, shares = kWave / lanes;
   const int d = (lane % lanes) * 4, left = a.D - d;
   const float unit = natural ? kLog2e : 1.0f;
+  const int bk = int(row / a.R), b = bk / a.K, kv = bk % a.K;
+  const Pieces pieces = pieces_of(a, __builtin_amdgcn_readfirstlane(b), keys);
+  const int64_t each = int64_t(a.K) * a.R, first = (int64_t(pieces.first) * a.K + kv) * a.R + row % a.R;
   float m = kLowest;
-  for (int s = lane; s < a.splits; s += kWave) m = fmaxf(m, a.part_stats[s * rows + row].x);
+  for (int s = lane; s < pieces.count; s += kWave) m = fmaxf(m, a.part_stats[first + s * each].x);
   for (int by = 32; by; by /= 2) m = fmaxf(m, __shfl_xor(m, by));
   float l = 0.0f, v[4] = {};
 #pragma unroll 4
-  for (int s = share; s < a.splits; s += shares) {
-    const float2 st = a.part_stats[s * rows + row];
+  for (int s = share; s < pieces.count; s += shares) {
+    const int64_t at = first + s * each;
+    const float2 st = a.part_stats[at];
     const float f = st.x == kLowest ? 0.0f : st.x == m ? 1.0f : __builtin_amdgcn_exp2f((st.x - m) * unit);
     l = fmaf(st.y, f, l);
-    const float* p = a.part + (s * rows + row) * a.D + d;
+    const float* p = a.part + at * a.D + d;
     if (a.D % 4 == 0) {
       f32x4 four = {0, 0, 0, 0};
       if (left > 0) four = *reinterpret_cast<const f32x4*>(p);
@@ -726,8 +799,7 @@ __global__ __launch_bounds__(256) void attention_combine_kernel(const Args a, in
   const float inverse = m == kLowest ? 0.0f : 1.0f / l;
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] *= inverse;
-  const int bk = int(row / a.R), b = bk / a.K;
-  const RowOf o = row_of(a, bk % a.K, uint32_t(row % a.R));
+  const RowOf o = row_of(a, kv, uint32_t(row % a.R));
   T* out = static_cast<T*>(a.out) + ((int64_t(b) * a.Q + o.query) * (a.K * a.G) + o.head) * a.D;
   store_four(out + d, v, left, a.out_vector);
   if (a.stats && lane == 0)
@@ -739,7 +811,7 @@ __global__ __launch_bounds__(256) void attention_combine_kernel(const Args a, in
 // It also leaves delta_i = do_i . o_i of its rows for the states' kernel.
 
 template <typename T, int DP, int MASK, int WR>
-__global__ __launch_bounds__(kThreads, (kGradQWaves<T, DP>)) void attention_grad_q_kernel(const Args a) {
+__global__ __launch_bounds__(kThreads, (kGradQWaves<T, DP, MASK>)) void attention_grad_q_kernel(const Args a) {
   using Shape = ForwardShape<T, DP, WR>;
   using TileT = Tile<T, DP>;
   constexpr int KB = Shape::KB, NB = DP / 32, kSteps = TileT::kPieces / 2, kKeys = Shape::kKeys;
@@ -749,6 +821,7 @@ __global__ __launch_bounds__(kThreads, (kGradQWaves<T, DP>)) void attention_grad
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int wr = wave % WR, wk = wave / WR;
   const KeyWalk<Shape> w(a);
+  if (w.b < 0) return;  // a slot that no image needs
   const uint32_t r = w.row_tile * Shape::kRows + 32 * wr + lane % 32;
   const bool live = r < a.R;
   const RowOf mine = row_of(a, w.kv, live ? r : a.R - 1);
@@ -778,7 +851,7 @@ __global__ __launch_bounds__(kThreads, (kGradQWaves<T, DP>)) void attention_grad
     delta = half_sum(delta);
   }
   const float2 stat = live ? a.row_stats[stat_at(a, w.b, mine)] : float2{INFINITY, 0.0f};
-  if (w.split == 0 && wk == 0 && live && lane < 32) a.delta[stat_at(a, w.b, mine)] = delta;
+  if (w.leads && wk == 0 && live && lane < 32) a.delta[stat_at(a, w.b, mine)] = delta;
 
   f32x16 acc[NB] = {};
   Scaled<T> scaled;
@@ -803,7 +876,7 @@ __global__ __launch_bounds__(kThreads, (kGradQWaves<T, DP>)) void attention_grad
       if constexpr (MASK == kBoolMask)
         if (!__any(mask[n].any() && live)) continue;
       float add[16];
-      if constexpr (MASK == kFloatMask) float_masks(a, mask_at, key0, w.states, add);
+      if constexpr (MASK == kFloatMask) float_masks(a, mask_at, key0, add);
       f32x16 s = {}, dp = {};
 #pragma unroll
       for (int t = 0; t < kSteps; ++t) {
@@ -820,7 +893,7 @@ __global__ __launch_bounds__(kThreads, (kGradQWaves<T, DP>)) void attention_grad
         if constexpr (MASK == kBoolMask) ds[i] = mask[n].on(i) ? ds[i] : 0.0f;
         if constexpr (MASK == kFloatMask) ds[i] = add[i] == kLowest ? 0.0f : ds[i];
       }
-      if (MASK == kNoMask && key0 + 32 > w.states) {
+      if (key0 + 32 > w.states) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) ds[i] = key0 + result_row(i) < w.states ? ds[i] : 0.0f;
       }
@@ -858,9 +931,9 @@ __global__ __launch_bounds__(kThreads, (kGradQWaves<T, DP>)) void attention_grad
     }
   }
   if (!live) return;
-  // A split's sums lie in grad_q's own order.
-  const int64_t elements = int64_t(a.B) * a.Q * a.K * a.G * a.D;
-  const int64_t out_at = ((int64_t(w.b) * a.Q + mine.query) * (a.K * a.G) + mine.head) * a.D;
+  // A piece's sums lie in the order of an image's grad_q.
+  const int64_t in_image = (int64_t(mine.query) * (a.K * a.G) + mine.head) * a.D;
+  const int64_t of_image = int64_t(a.Q) * (a.K * a.G) * a.D;
 #pragma unroll
   for (int c = 0; c < NB; ++c)
 #pragma unroll
@@ -868,9 +941,9 @@ __global__ __launch_bounds__(kThreads, (kGradQWaves<T, DP>)) void attention_grad
       const int d = 32 * c + 8 * g + 4 * (lane / 32);
       const float v[4] = {acc[c][4 * g], acc[c][4 * g + 1], acc[c][4 * g + 2], acc[c][4 * g + 3]};
       if (a.splits > 1)
-        store_four(a.part + w.split * elements + out_at + d, v, a.D - d, a.D % 4 == 0);
+        store_four(a.part + w.slot * of_image + in_image + d, v, a.D - d, a.D % 4 == 0);
       else
-        store_four(static_cast<T*>(a.grad_q) + out_at + d, v, a.D - d, a.out_vector);
+        store_four(static_cast<T*>(a.grad_q) + w.b * of_image + in_image + d, v, a.D - d, a.out_vector);
     }
 }
 
@@ -898,7 +971,7 @@ __device__ inline uint32_t byte_bits(uint32_t four) {
 }
 
 template <typename T, int DP, int MASK>
-__global__ __launch_bounds__(kThreads, (kGradStatesWaves<T, DP>)) void attention_grad_states_kernel(const Args a) {
+__global__ __launch_bounds__(kThreads, (kGradStatesWaves<T, DP, MASK>)) void attention_grad_states_kernel(const Args a) {
   using Shape = StatesShape<T, DP>;
   using TileT = Tile<T, DP>;
   constexpr int NB = DP / 32, kSteps = TileT::kPieces / 2, kRows = Shape::kRows;
@@ -906,13 +979,18 @@ __global__ __launch_bounds__(kThreads, (kGradStatesWaves<T, DP>)) void attention
   __shared__ __attribute__((aligned(16))) char lds[Shape::kLds];
 
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  // The heads whose rows share a cache line first (the key heads are a multiple of `near`),
+  // then the tiles, which read the same queries.
   const uint32_t key_tiles = (uint32_t(a.S) + Shape::kKeys - 1) / Shape::kKeys;
   uint32_t id = xcd_order(blockIdx.x, gridDim.x);
+  int kv = int(id % uint32_t(a.near));
+  id /= a.near;
   const int key_tile = int(id % key_tiles);
   id /= key_tiles;
   const int split = int(id % uint32_t(a.row_splits));
-  const int bk = int(id / uint32_t(a.row_splits));
-  const int b = bk / a.K, kv = bk % a.K;
+  id /= a.row_splits;
+  kv += int(id % uint32_t(a.K / a.near)) * a.near;
+  const int b = int(id / uint32_t(a.K / a.near));
 
   const int states = __builtin_amdgcn_readfirstlane(states_of(a, b));
   const int key = key_tile * Shape::kKeys + 32 * wave + lane % 32;
@@ -955,26 +1033,16 @@ __global__ __launch_bounds__(kThreads, (kGradStatesWaves<T, DP>)) void attention
       const int row = threadIdx.x / kWaves, k0 = key_tile * Shape::kKeys + 32 * int(threadIdx.x % kWaves);
       const int64_t at = mask_row_at(a, b, RowOf{query + (row < left ? row : left - 1), head});
       const uint8_t* bytes = static_cast<const uint8_t*>(a.mask) + at;
-      if (a.mask_words && k0 + 32 <= states) {
+      if (k0 + 32 <= a.mask_row_keys) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const u32x4 four = *reinterpret_cast<const u32x4*>(bytes + k0 + 16 * i);
+          const u32x4 four = load_anywhere<u32x4>(bytes + k0 + 16 * i);
 #pragma unroll
           for (int j = 0; j < 4; ++j) raw[4 * i + j] = four[j];
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int k1 = k0 + 4 * i;
-          raw[i] = 0;
-          if (a.mask_quads && k1 + 4 <= states) {
-            raw[i] = *reinterpret_cast<const uint32_t*>(bytes + k1);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (k1 + j < states) raw[i] |= uint32_t(bytes[int64_t(k1 + j) * a.mask_key] != 0) << (8 * j);
-          }
-        }
+        for (int i = 0; i < 8; ++i) raw[i] = four_bytes(a, bytes, k0 + 4 * i);
       }
     }
     if (++next_tile == query_tiles) {
@@ -1043,7 +1111,7 @@ __global__ __launch_bounds__(kThreads, (kGradStatesWaves<T, DP>)) void attention
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int row = local + result_row(i);
-          add[i] = on && row < float_rows ? float_mask(a, float_at + row * a.mask_row + int64_t(key) * a.mask_key) : kLowest;
+          add[i] = on && row < float_rows ? float_mask(a, float_at + row * a.mask_row + key) : kLowest;
         }
       }
       f32x16 s = {}, dp;
@@ -1118,32 +1186,62 @@ __global__ __launch_bounds__(kThreads, (kGradStatesWaves<T, DP>)) void attention
     }
 }
 
-// out = the sum of `count` fp32 parts of n elements each, in their order.
+// out = the sum of fp32 parts of n elements each, in a fixed order: for grad_q (`of_keys` keys in
+// a tile) the parts of image blockIdx.y's pieces, for the states all row_splits parts of grad_k
+// (blockIdx.y 0) and grad_v. Four waves share the parts of 64 x 4 elements.
 template <typename T>
-__global__ __launch_bounds__(256) void attention_sum_kernel(const float* part, int count, int64_t n, T* out,
-                                                            const float* part2, T* out2) {
-  const int64_t at = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4;
-  if (at >= n) return;
-  if (blockIdx.y) {
-    part = part2;
-    out = out2;
+__global__ __launch_bounds__(kThreads) void attention_sum_kernel(const Args a, int64_t n, int of_keys) {
+  __shared__ f32x4 sums[kWaves - 1][kWave];
+  const int lane = threadIdx.x % kWave, share = threadIdx.x / kWave;
+  const int64_t at = (int64_t(blockIdx.x) * kWave + lane) * 4;
+  const float* part;
+  T* out;
+  Pieces pieces = {0, a.row_splits};
+  if (of_keys) {
+    pieces = pieces_of(a, int(blockIdx.y), of_keys);
+    part = a.part;
+    out = static_cast<T*>(a.grad_q) + blockIdx.y * n;
+  } else {
+    part = blockIdx.y ? a.part_v : a.part_k;
+    out = static_cast<T*>(blockIdx.y ? a.grad_v : a.grad_k);
   }
-  float v[4] = {};
   const bool vector = n % 4 == 0;
+  f32x4 v = {0, 0, 0, 0};
+  if (at < n) {
 #pragma unroll 4
-  for (int s = 0; s < count; ++s) {
-    const float* p = part + s * n + at;
-    if (vector) {
-      const f32x4 four = *reinterpret_cast<const f32x4*>(p);
+    for (int s = pieces.first + share; s < pieces.first + pieces.count; s += kWaves) {
+      const float* p = part + s * n + at;
+      if (vector) {
+        v += *reinterpret_cast<const f32x4*>(p);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += four[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (at + i < n) v[i] += p[i];
+        for (int i = 0; i < 4; ++i)
+          if (at + i < n) v[i] += p[i];
+      }
     }
   }
-  store_four(out + at, v, int(n - at < 4 ? n - at : 4), vector && reinterpret_cast<uintptr_t>(out) % 16 == 0);
+  if (share) sums[share - 1][lane] = v;
+  __syncthreads();
+  if (share || at >= n) return;
+#pragma unroll
+  for (int s = 0; s < kWaves - 1; ++s) v += sums[s][lane];
+  const float four[4] = {v[0], v[1], v[2], v[3]};
+  store_four(out + at, four, int(n - at < 4 ? n - at : 4), vector && reinterpret_cast<uintptr_t>(out) % 16 == 0);
+}
+
+// A mask whose keys do not lie side by side, or of fewer than 4, as rows of `keys` (a multiple
+// of 32), with zeros past S: one thread for each element. Axes of stride 0 have size 1.
+template <typename V>
+__global__ __launch_bounds__(256) void attention_pack_mask_kernel(const V* from, V* to, int64_t batch, int64_t head,
+                                                                  int64_t row, int64_t key, int heads, int rows, int S,
+                                                                  int keys, int64_t elements) {
+  const int64_t n = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (n >= elements) return;
+  const int k = int(n % keys);
+  int64_t at = n / keys;
+  const int64_t r = at % rows;
+  at /= rows;
+  to[n] = k < S ? from[(at / heads) * batch + (at % heads) * head + r * row + k * key] : V(0);
 }
 
 // Rows of D channels at any strides and alignment, as dense rows of Dp with zeros past D: one
@@ -1210,7 +1308,7 @@ template <typename T> void launch_forward(const Args& a, int mask_kind, bool few
     int lanes = 1;
     while (4 * lanes < a.D) lanes *= 2;
     attention_combine_kernel<T><<<uint32_t(ceil_div(int64_t(a.B) * a.K * a.R, kWaves)), kThreads, 0, s>>>(
-        a, lanes, mask_kind == kFloatMask);
+        a, lanes, mask_kind == kFloatMask, few_rows ? 128 : 64);
   }
 }
 
@@ -1230,14 +1328,13 @@ void launch_backward(const Args& a, int mask_kind, bool few_rows, uint32_t group
     });
   });
   if (groups && a.splits > 1) {
-    const int64_t count = int64_t(a.B) * a.Q * a.K * a.G * a.D;
-    attention_sum_kernel<T><<<uint32_t(ceil_div(count, 1024)), 256, 0, s>>>(
-        a.part, a.splits, count, static_cast<T*>(a.grad_q), nullptr, nullptr);
+    const int64_t n = int64_t(a.Q) * a.K * a.G * a.D;
+    attention_sum_kernel<T><<<dim3(uint32_t(ceil_div(n, 4 * kWave)), uint32_t(a.B)), kThreads, 0, s>>>(
+        a, n, few_rows ? 128 : 64);
   }
   if (key_groups && a.row_splits > 1) {
-    const int64_t count = int64_t(a.B) * a.S * a.K * a.D;
-    attention_sum_kernel<T><<<dim3(uint32_t(ceil_div(count, 1024)), 2), 256, 0, s>>>(
-        a.part_k, a.row_splits, count, static_cast<T*>(a.grad_k), a.part_v, static_cast<T*>(a.grad_v));
+    const int64_t n = int64_t(a.B) * a.S * a.K * a.D;
+    attention_sum_kernel<T><<<dim3(uint32_t(ceil_div(n, 4 * kWave)), 2), kThreads, 0, s>>>(a, n, 0);
   }
 }
 

@@ -29,11 +29,12 @@ struct Packed {
 
 struct Plan {
   bool few_rows;   // one row tile of 32: the waves share the rows
-  int splits;      // of the keys
+  int splits;      // of an image's keys
+  bool balanced;   // splits by the images' lengths
   int row_splits;  // of the rows, in the states' kernel
   int64_t forward_bytes, backward_bytes;
   int64_t delta_at, part_at, part_stats_at, part_k_at, part_v_at;
-  Packed q, k, v, o, go;
+  Packed q, k, v, o, go, mask;
 };
 
 // `grad_output` and the output are dense: one packing rule for both by alignment (the size
@@ -46,6 +47,7 @@ Plan plan_of(const deformops_attention& c) {
   const int64_t rows = p.few_rows ? 32 : 128, keys = p.few_rows ? 128 : 64;
   const int64_t groups = BK * ceil_div(R, rows), tiles = ceil_div(c.keys, keys);
   p.splits = int(std::max<int64_t>(1, std::min<int64_t>(ceil_div(kWanted, std::max<int64_t>(1, groups)), tiles / 2)));
+  p.balanced = p.splits > 1 && c.key_lengths && c.batch > 1 && c.batch <= 64;
   const int64_t row_tile = DP * size <= 192 ? 64 : 32;
   const int64_t key_groups = BK * ceil_div(c.keys, 128), row_tiles = G * ceil_div(c.queries, row_tile);
   p.row_splits = int(std::max<int64_t>(1, std::min<int64_t>(ceil_div(kWanted, std::max<int64_t>(1, key_groups)), row_tiles / 2)));
@@ -63,6 +65,10 @@ Plan plan_of(const deformops_attention& c) {
   p.q = pack(rows_as_they_are(c, c.query, c.query_strides, c.queries), c.queries, c.heads);
   p.k = pack(rows_as_they_are(c, c.key, c.key_strides, c.keys), c.keys, c.key_heads);
   p.v = pack(rows_as_they_are(c, c.value, c.value_strides, c.keys), c.keys, c.key_heads);
+  const int64_t (&m)[4] = c.mask_strides;
+  if (c.mask_kind != kNoMask && c.keys && (m[3] != 1 || c.keys < 4))
+    p.mask = Packed{true, take((m[0] ? c.batch : 1) * (m[1] ? c.heads : 1) * (m[2] ? c.queries : 1) *
+                               ceil_div(c.keys, 32) * 32 * (c.mask_kind == kBoolMask ? 1 : element_size(c.mask_dtype)))};
   p.part_at = take(p.splits > 1 ? p.splits * BK * R * c.channels * 4 : 0);
   const int64_t shared = at;
   p.part_stats_at = take(p.splits > 1 ? p.splits * BK * R * 8 : 0);
@@ -126,20 +132,33 @@ Args args_of(const deformops_attention& c, const Plan& p, void* workspace, hipSt
   a.q = rows_of(c, c.query, c.query_strides, p.q, c.queries, c.heads, ws, s);
   a.k = rows_of(c, c.key, c.key_strides, p.k, c.keys, c.key_heads, ws, s);
   a.v = rows_of(c, c.value, c.value_strides, p.v, c.keys, c.key_heads, ws, s);
-  if (c.mask_kind != kNoMask) {
-    const int size = c.mask_kind == kBoolMask ? 1 : element_size(c.mask_dtype);
+  if (c.mask_kind != kNoMask && c.keys) {
+    const int64_t (&m)[4] = c.mask_strides;
     a.mask = c.mask;
-    a.mask_batch = c.mask_strides[0]; a.mask_head = c.mask_strides[1];
-    a.mask_row = c.mask_strides[2]; a.mask_key = c.mask_strides[3];
+    a.mask_batch = m[0]; a.mask_head = m[1]; a.mask_row = m[2]; a.mask_key = m[3];
+    a.mask_row_keys = int(c.keys);
     a.mask_type = c.mask_dtype;
-    auto together = [&](int64_t n) {
-      return c.mask_strides[3] == 1 && aligned(c.mask, size_t(n) * size) && c.mask_strides[0] % n == 0 &&
-             c.mask_strides[1] % n == 0 && c.mask_strides[2] % n == 0;
-    };
-    a.mask_quads = together(4);
-    a.mask_words = together(16);
-    a.mask_of_keys = c.mask_kind == kBoolMask && (c.mask_strides[1] == 0 || c.heads == 1) &&
-                     (c.mask_strides[2] == 0 || c.queries == 1);
+    a.mask_of_keys = c.mask_kind == kBoolMask && (m[1] == 0 || c.heads == 1) && (m[2] == 0 || c.queries == 1);
+    if (p.mask.on) {
+      const int64_t keys = ceil_div(c.keys, 32) * 32;
+      const int64_t images = m[0] ? c.batch : 1, heads = m[1] ? c.heads : 1, rows = m[2] ? c.queries : 1;
+      const int64_t elements = images * heads * rows * keys;
+      a.mask = ws + p.mask.at;
+      a.mask_batch = m[0] ? heads * rows * keys : 0;
+      a.mask_head = m[1] ? rows * keys : 0;
+      a.mask_row = m[2] ? keys : 0;
+      a.mask_key = 1;
+      a.mask_row_keys = int(keys);
+      auto pack = [&](auto v) {
+        using V = decltype(v);
+        attention_pack_mask_kernel<V><<<uint32_t(ceil_div(elements, 256)), 256, 0, s>>>(
+            static_cast<const V*>(c.mask), reinterpret_cast<V*>(ws + p.mask.at), m[0], m[1], m[2], m[3], int(heads), int(rows),
+            int(c.keys), int(keys), elements);
+      };
+      if (c.mask_kind == kBoolMask) pack(uint8_t());
+      else if (c.mask_dtype == MSDA_F32) pack(uint32_t());
+      else pack(uint16_t());
+    }
   }
   a.lengths = c.key_lengths;
   a.lengths_i64 = c.index_dtype == MSDA_I64;
@@ -151,6 +170,10 @@ Args args_of(const deformops_attention& c, const Plan& p, void* workspace, hipSt
   a.R = uint32_t(c.queries * a.G);
   a.scale = c.scale;
   a.splits = p.splits;
+  a.slots = p.splits * a.B;
+  a.balanced = p.balanced;
+  const int row_bytes = a.D * element_size(c.dtype);
+  for (a.near = 1; a.near * row_bytes < 128 && a.K % (2 * a.near) == 0; a.near *= 2) {}
   a.row_splits = p.row_splits;
   a.part = reinterpret_cast<float*>(ws + p.part_at);
   a.part_stats = reinterpret_cast<float2*>(ws + p.part_stats_at);
