@@ -417,12 +417,15 @@ struct All {
 };
 
 // Two waves of a SIMD hide each other's waits where their registers allow it (256 each).
-template <typename T, int DP, int MASK> constexpr int kForwardWaves =
-    sizeof(T) == 4 ? (DP > 64 ? 1 : 2) : DP == 32 ? (MASK ? 3 : 4) : DP == 64 ? (MASK ? 2 : 3) : DP == 128 && MASK ? 1 : 2;
-template <typename T, int DP, int MASK> constexpr int kGradQWaves =
-    sizeof(T) == 4 ? (DP > 32 ? 1 : 2) : DP == 32 ? 3 : DP <= (MASK ? 64 : 96) ? 2 : 1;
-template <typename T, int DP, int MASK> constexpr int kGradStatesWaves =
-    sizeof(T) == 4 ? (DP > 32 ? 1 : 2) : DP == 32 ? (MASK ? 2 : 3) : DP == 64 ? 2 : 1;
+constexpr int forward_waves(int size, int DP, int mask) {
+  return size == 4 ? (DP > 64 ? 1 : 2) : DP == 32 ? (mask ? 3 : 4) : DP == 64 ? (mask ? 2 : 3) : DP == 128 && mask ? 1 : 2;
+}
+constexpr int grad_q_waves(int size, int DP, int mask) {
+  return size == 4 ? (DP > 32 ? 1 : 2) : DP == 32 ? 3 : DP <= (mask ? 64 : 96) ? 2 : 1;
+}
+constexpr int grad_states_waves(int size, int DP, int mask) {
+  return size == 4 ? (DP > 32 ? 1 : 2) : DP == 32 ? (mask ? 2 : 3) : DP == 64 ? 2 : 1;
+}
 
 // ---------------------------------------------------------------------------
 // Forward. A workgroup has 4 waves: WR of them along the rows (32 each), 4 / WR along the keys
@@ -435,7 +438,7 @@ template <typename T, int DP, int WR> struct ForwardShape {
   static constexpr int kRows = 32 * WR;
   static constexpr int kKeys = 32 * KB * WK;
   static constexpr int kTile = kKeys * Tile<T, DP>::kRowBytes;
-  static constexpr int kBuffers = 4 * kTile <= (kForwardWaves<T, DP, kNoMask> > 1 ? 80 : 128) * 1024 ? 2 : 1;
+  static constexpr int kBuffers = 4 * kTile <= (forward_waves(sizeof(T), DP, kNoMask) > 1 ? 80 : 128) * 1024 ? 2 : 1;
   static constexpr int kJoin = WK > 1 ? WK * 32 * WR * (DP + 2) * 4 : 0;
   static constexpr int kLds = std::max(2 * kBuffers * kTile, kJoin);
 };
@@ -580,7 +583,7 @@ template <typename T, int DP, int MASK, typename Shape> struct KeyStage {
 };
 
 template <typename T, int DP, int MASK, int WR>
-__global__ __launch_bounds__(kThreads, (kForwardWaves<T, DP, MASK>)) void attention_forward_kernel(const Args a) {
+__global__ __launch_bounds__(kThreads, forward_waves(sizeof(T), DP, MASK)) void attention_forward_kernel(const Args a) {
   using Shape = ForwardShape<T, DP, WR>;
   using TileT = Tile<T, DP>;
   constexpr int KB = Shape::KB, NB = DP / 32, kSteps = TileT::kPieces / 2, kKeys = Shape::kKeys;
@@ -768,27 +771,47 @@ __global__ __launch_bounds__(256) void attention_combine_kernel(const Args a, in
   const int bk = int(row / a.R), b = bk / a.K, kv = bk % a.K;
   const Pieces pieces = pieces_of(a, __builtin_amdgcn_readfirstlane(b), keys);
   const int64_t each = int64_t(a.K) * a.R, first = (int64_t(pieces.first) * a.K + kv) * a.R + row % a.R;
-  float m = kLowest;
-  for (int s = lane; s < pieces.count; s += kWave) m = fmaxf(m, a.part_stats[first + s * each].x);
-  for (int by = 32; by; by /= 2) m = fmaxf(m, __shfl_xor(m, by));
-  float l = 0.0f, v[4] = {};
-#pragma unroll 4
-  for (int s = share; s < pieces.count; s += shares) {
-    const int64_t at = first + s * each;
-    const float2 st = a.part_stats[at];
-    const float f = st.x == kLowest ? 0.0f : st.x == m ? 1.0f : __builtin_amdgcn_exp2f((st.x - m) * unit);
-    l = fmaf(st.y, f, l);
-    const float* p = a.part + at * a.D + d;
+  auto four_at = [&](int s) __attribute__((always_inline)) {
+    const float* p = a.part + (first + s * each) * a.D + d;
+    f32x4 v = {0, 0, 0, 0};
+    if (s >= pieces.count || left <= 0) return v;
     if (a.D % 4 == 0) {
-      f32x4 four = {0, 0, 0, 0};
-      if (left > 0) four = *reinterpret_cast<const f32x4*>(p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = fmaf(four[i], f, v[i]);
+      v = *reinterpret_cast<const f32x4*>(p);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (i < left) v[i] = fmaf(p[i], f, v[i]);
+        if (i < left) v[i] = p[i];
     }
+    return v;
+  };
+  // Statistics of up to 64 pieces, one in a lane, and the first rows of their sums: all loads at
+  // once. Calls of more pieces go on in turns of 64.
+  constexpr int kAhead = 4;
+  float m = kLowest, l = 0.0f, v[4] = {};
+  for (int turn = 0; turn < pieces.count; turn += kWave) {
+    const int here = min(pieces.count - turn, kWave);
+    const float2 st = lane < here ? a.part_stats[first + (turn + lane) * each] : float2{kLowest, 0.0f};
+    f32x4 ahead[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) ahead[i] = four_at(turn + share + i * shares);
+    float top = fmaxf(m, st.x);
+    for (int by = 32; by; by /= 2) top = fmaxf(top, __shfl_xor(top, by));
+    const float old = m == kLowest ? 0.0f : __builtin_amdgcn_exp2f((m - top) * unit);
+    const float mine = st.x == kLowest ? 0.0f : st.x == top ? 1.0f : __builtin_amdgcn_exp2f((st.x - top) * unit);
+    l *= old;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] *= old;
+    m = top;
+    auto add = [&](int s, f32x4 four) __attribute__((always_inline)) {
+      const float f = __shfl(mine, s), sum = __shfl(st.y, s);
+      if (s >= here) return;
+      l = fmaf(sum, f, l);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = fmaf(four[i], f, v[i]);
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) add(share + i * shares, ahead[i]);
+    for (int s = kAhead * shares; s < here; s += shares) add(share + s, share + s < here ? four_at(turn + share + s) : f32x4{0, 0, 0, 0});
   }
   for (int by = lanes; by < kWave; by *= 2) {
     l += __shfl_xor(l, by);
@@ -811,7 +834,7 @@ __global__ __launch_bounds__(256) void attention_combine_kernel(const Args a, in
 // It also leaves delta_i = do_i . o_i of its rows for the states' kernel.
 
 template <typename T, int DP, int MASK, int WR>
-__global__ __launch_bounds__(kThreads, (kGradQWaves<T, DP, MASK>)) void attention_grad_q_kernel(const Args a) {
+__global__ __launch_bounds__(kThreads, grad_q_waves(sizeof(T), DP, MASK)) void attention_grad_q_kernel(const Args a) {
   using Shape = ForwardShape<T, DP, WR>;
   using TileT = Tile<T, DP>;
   constexpr int KB = Shape::KB, NB = DP / 32, kSteps = TileT::kPieces / 2, kKeys = Shape::kKeys;
@@ -971,7 +994,7 @@ __device__ inline uint32_t byte_bits(uint32_t four) {
 }
 
 template <typename T, int DP, int MASK>
-__global__ __launch_bounds__(kThreads, (kGradStatesWaves<T, DP, MASK>)) void attention_grad_states_kernel(const Args a) {
+__global__ __launch_bounds__(kThreads, grad_states_waves(sizeof(T), DP, MASK)) void attention_grad_states_kernel(const Args a) {
   using Shape = StatesShape<T, DP>;
   using TileT = Tile<T, DP>;
   constexpr int NB = DP / 32, kSteps = TileT::kPieces / 2, kRows = Shape::kRows;

@@ -7,7 +7,7 @@ namespace {
 
 using namespace attention;
 
-constexpr int kWanted = 512;  // workgroups that fill 256 CUs twice
+constexpr int64_t kCus = 256;
 
 int element_size(int dtype) { return dtype == MSDA_F32 ? 4 : dtype == MSDA_F16 || dtype == MSDA_BF16 ? 2 : 0; }
 
@@ -46,11 +46,19 @@ Plan plan_of(const deformops_attention& c) {
   p.few_rows = R <= 64 && size * DP < 512;
   const int64_t rows = p.few_rows ? 32 : 128, keys = p.few_rows ? 128 : 64;
   const int64_t groups = BK * ceil_div(R, rows), tiles = ceil_div(c.keys, keys);
-  p.splits = int(std::max<int64_t>(1, std::min<int64_t>(ceil_div(kWanted, std::max<int64_t>(1, groups)), tiles / 2)));
+  // Pieces of the key axis (of the rows, in the states' kernel) for as many workgroups as the
+  // card holds at once: one more would wait for a whole turn.
+  auto pieces = [](int64_t groups, int waves, int64_t tiles) {
+    return int(std::max<int64_t>(1, std::min<int64_t>(kCus * waves / std::max<int64_t>(1, groups), tiles / 2)));
+  };
+  // The LDS of a workgroup whose waves share the rows (ForwardShape), in KB of a CU's 160.
+  const int tile = DP * size / 8, lds = 4 * tile <= 80 ? 4 * tile : std::max(2 * tile, DP / 2 + 1);
+  const int lds_waves = p.few_rows ? 160 / lds : 4;
+  p.splits = pieces(groups, std::min(lds_waves, forward_waves(size, DP, c.mask_kind)), tiles);
   p.balanced = p.splits > 1 && c.key_lengths && c.batch > 1 && c.batch <= 64;
   const int64_t row_tile = DP * size <= 192 ? 64 : 32;
   const int64_t key_groups = BK * ceil_div(c.keys, 128), row_tiles = G * ceil_div(c.queries, row_tile);
-  p.row_splits = int(std::max<int64_t>(1, std::min<int64_t>(ceil_div(kWanted, std::max<int64_t>(1, key_groups)), row_tiles / 2)));
+  p.row_splits = pieces(key_groups, grad_states_waves(size, DP, c.mask_kind), row_tiles);
 
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
