@@ -58,9 +58,12 @@ struct Rows {
 
 struct Args {
   Rows q, k, v;
+  // A bool mask as words of 32 keys each (bit k % 32 of word k / 32, zeros past S; mask_bits_kernel),
+  // a float mask as it is, its keys side by side. Strides of the image, the head and the row, 0
+  // where it is one for all.
   const void* mask;
-  int64_t mask_batch, mask_head, mask_row, mask_key;
-  int mask_row_keys;  // keys of a mask's row in memory, side by side (at least 4)
+  int64_t mask_batch, mask_head, mask_row;
+  int mask_row_keys;  // keys of a float mask's row in memory (at least 4)
   int mask_type;      // element type of a float mask
   bool mask_of_keys;  // a bool mask that is one for all rows and heads: it removes states
   const void* lengths;
@@ -281,7 +284,10 @@ __device__ inline float float_mask(const Args& a, int64_t at) {
   if (a.mask_type == MSDA_BF16) return widen(static_cast<const bf16_t*>(a.mask)[at]);
   return widen(static_cast<const f16_t*>(a.mask)[at]);
 }
-__device__ inline bool bool_mask(const Args& a, int64_t at) { return static_cast<const uint8_t*>(a.mask)[at] != 0; }
+// One key's bit of a mask of states.
+__device__ inline bool state_bit(const Args& a, int b, int key) {
+  return (static_cast<const uint32_t*>(a.mask)[b * a.mask_batch + key / 32] >> (key % 32)) & 1;
+}
 
 // Mask rows may begin at any byte: global loads take any alignment.
 template <typename V> __device__ inline V load_anywhere(const void* p) {
@@ -289,32 +295,14 @@ template <typename V> __device__ inline V load_anywhere(const void* p) {
   return static_cast<const Any*>(p)->v;
 }
 
-// Four bytes of a mask's row from key k0: keys past the row are 0.
-__device__ inline uint32_t four_bytes(const Args& a, const uint8_t* row, int k0) {
-  const int at = min(k0, a.mask_row_keys - 4), past = k0 - at;
-  const uint32_t four = load_anywhere<uint32_t>(row + at);
-  return past > 3 ? 0 : four >> (8 * past);
-}
+// The bits of the 16 result rows in a lane's word of 32 keys: result row r in bit
+// 8 (r / 4) + r % 4.
+__device__ inline uint32_t result_bits(uint32_t word) { return word >> (4 * (int(threadIdx.x % kWave) / 32)); }
 
-// A bool mask's bytes for the 16 result rows (32 keys from `key`) of the row whose first mask
-// element is `at`: four words, result row r in byte r % 4 of word r / 4.
-struct MaskBytes {
-  uint32_t word[4];
-  __device__ bool any() const { return (word[0] | word[1] | word[2] | word[3]) != 0; }
-  __device__ bool on(int r) const { return ((word[r / 4] >> (8 * (r % 4))) & 0xff) != 0; }
-};
-__device__ __forceinline__ MaskBytes mask_bytes(const Args& a, int64_t at, int key) {
-  MaskBytes out;
-  const uint8_t* row = static_cast<const uint8_t*>(a.mask) + at;
-  const int k0 = key + 4 * (int(threadIdx.x % kWave) / 32);
-  if (key + 32 <= a.mask_row_keys) {
-#pragma unroll
-    for (int g = 0; g < 4; ++g) out.word[g] = load_anywhere<uint32_t>(row + k0 + 8 * g);
-  } else {
-#pragma unroll
-    for (int g = 0; g < 4; ++g) out.word[g] = four_bytes(a, row, k0 + 8 * g);
-  }
-  return out;
+// v where bit `bit` of `bits` is set, else `other`.
+__device__ inline float where_bit(uint32_t bits, int bit, float v, float other) {
+  const uint32_t all = uint32_t(int32_t(bits << (31 - bit)) >> 31);
+  return __uint_as_float((all & __float_as_uint(v)) | (~all & __float_as_uint(other)));
 }
 
 // The additive mask of the 16 result rows; 0 past the row.
@@ -553,7 +541,7 @@ template <typename T, int DP, int MASK, typename Shape> struct KeyStage {
   const T *k_base, *v_base;
   int64_t mask_at;
   int local;  // this wave's first key in a tile
-  MaskBytes next[KB];
+  uint32_t next[KB];  // this row's mask words
 
   __device__ KeyStage(const Args& args, const KeyWalk<Shape>& walk, int64_t mask, int first_key)
       : a(args), w(walk), mask_at(mask), local(first_key) {
@@ -567,7 +555,7 @@ template <typename T, int DP, int MASK, typename Shape> struct KeyStage {
     const T *ks = k_base + int64_t(key) * a.k.row, *vs = v_base + int64_t(key) * a.v.row;
     if (MASK == kBoolMask && a.mask_of_keys) {  // removed states are read as zeros
       auto kept = [&](int row) {
-        return row < left && bool_mask(a, w.b * a.mask_batch + int64_t(key + row) * a.mask_key);
+        return row < left && state_bit(a, w.b, key + row);
       };
       k.load(ks, left, kept);
       v.load(vs, left, kept);
@@ -577,7 +565,8 @@ template <typename T, int DP, int MASK, typename Shape> struct KeyStage {
     }
     if constexpr (MASK == kBoolMask) {
 #pragma unroll
-      for (int n = 0; n < KB; ++n) next[n] = mask_bytes(a, mask_at, key + local + 32 * n);
+      for (int n = 0; n < KB; ++n)
+        next[n] = static_cast<const uint32_t*>(a.mask)[mask_at + (key + local) / 32 + n];
     }
   }
 };
@@ -622,31 +611,32 @@ __global__ __launch_bounds__(kThreads, forward_waves(sizeof(T), DP, MASK)) void 
     if (Shape::kBuffers == 1 && tile > w.first) __syncthreads();
     stage.k.store(k_tile);
     stage.v.store(v_tile);
-    MaskBytes mask[KB];
+    uint32_t mask[KB];
 #pragma unroll
-    for (int n = 0; n < KB; ++n) mask[n] = stage.next[n];
+    for (int n = 0; n < KB; ++n) mask[n] = MASK == kBoolMask ? stage.next[n] : 0;
     __syncthreads();
     if (tile + 1 < w.last) stage.load(tile + 1);
 
     const int key0 = tile * kKeys + local;  // this wave's keys
     if constexpr (MASK == kBoolMask) {
-      bool any = false;
+      uint32_t any = 0;
 #pragma unroll
-      for (int n = 0; n < KB; ++n) any |= mask[n].any();
-      if (!__any(any && live)) return;
+      for (int n = 0; n < KB; ++n) any |= mask[n];
+      if (!__any(any != 0 && live)) return;
     }
     float x[KB][16];
 #pragma unroll
     for (int n = 0; n < KB; ++n) {
       float add[16];
       if constexpr (MASK == kFloatMask) float_masks(a, mask_at, key0 + 32 * n, add);
+      const uint32_t bits = result_bits(mask[n]);
       f32x16 s = {};
 #pragma unroll
       for (int t = 0; t < kSteps; ++t) s = Mma<T>::rows(row_piece<T, DP>(k_tile, local + 32 * n, t), q[t], s);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         x[n][i] = s[i];
-        if constexpr (MASK == kBoolMask) x[n][i] = mask[n].on(i) ? s[i] : kLowest;
+        if constexpr (MASK == kBoolMask) x[n][i] = where_bit(bits, 8 * (i / 4) + i % 4, s[i], kLowest);
         if constexpr (MASK == kFloatMask) x[n][i] = add[i] == kLowest ? kLowest : fmaf(s[i], factor, add[i]);
       }
     }
@@ -757,74 +747,84 @@ __global__ __launch_bounds__(kThreads, forward_waves(sizeof(T), DP, MASK)) void 
     }
 }
 
-// Joins the splits of the forward. A row has `lanes` lanes (a power of two) of four channels
-// each, and 64 / lanes of them in a wave share its splits, so that few rows of many splits do
-// not wait for one lane's loads in turn.
+// Joins the pieces of the forward's rows. A row has `lanes` lanes of four channels each, `shares`
+// of them (both powers of two) for its pieces: a lane takes every shares-th piece, four at a time,
+// and the shares meet in LDS in their order. So few rows of many pieces do not wait for one
+// lane's loads in turn, and many rows of few pieces fill the workgroup.
 template <typename T>
-__global__ __launch_bounds__(256) void attention_combine_kernel(const Args a, int lanes, bool natural, int keys) {
-  const int64_t rows = int64_t(a.B) * a.K * a.R;
-  const int64_t row = int64_t(blockIdx.x) * kWaves + threadIdx.x / kWave;
-  if (row >= rows) return;  // whole waves
-  const int lane = threadIdx.x % kWave, share = lane / lanes, shares = kWave / lanes;
-  const int d = (lane % lanes) * 4, left = a.D - d;
+__global__ __launch_bounds__(kThreads) void attention_combine_kernel(const Args a, int lanes, int shares, bool natural,
+                                                                     int keys) {
+  __shared__ f32x4 sums[kThreads];
+  __shared__ float2 stats[kThreads];
+  const int b = int(blockIdx.y) / a.K, kv = int(blockIdx.y) % a.K;
+  const Pieces pieces = pieces_of(a, b, keys);
+  const int rows = kThreads / (lanes * shares);  // of this workgroup
+  const int lane = int(threadIdx.x) % lanes, share = (int(threadIdx.x) / lanes) % shares;
+  const int64_t r = int64_t(blockIdx.x) * rows + int(threadIdx.x) / (lanes * shares);
+  const bool live = r < a.R;
+  const int d = lane * 4, left = a.D - d;
   const float unit = natural ? kLog2e : 1.0f;
-  const int bk = int(row / a.R), b = bk / a.K, kv = bk % a.K;
-  const Pieces pieces = pieces_of(a, __builtin_amdgcn_readfirstlane(b), keys);
-  const int64_t each = int64_t(a.K) * a.R, first = (int64_t(pieces.first) * a.K + kv) * a.R + row % a.R;
-  auto four_at = [&](int s) __attribute__((always_inline)) {
-    const float* p = a.part + (first + s * each) * a.D + d;
-    f32x4 v = {0, 0, 0, 0};
-    if (s >= pieces.count || left <= 0) return v;
-    if (a.D % 4 == 0) {
-      v = *reinterpret_cast<const f32x4*>(p);
-    } else {
+  const int64_t each = int64_t(a.K) * a.R, first = (int64_t(pieces.first) * a.K + kv) * a.R + r;
+  float m = kLowest, l = 0.0f;
+  f32x4 v = {0, 0, 0, 0};
+  auto join = [&](const float2& st, f32x4 four, float top) __attribute__((always_inline)) {
+    const float f = st.x == kLowest ? 0.0f : __builtin_amdgcn_exp2f((st.x - top) * unit);
+    l = fmaf(st.y, f, l);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i < left) v[i] = p[i];
-    }
-    return v;
+    for (int i = 0; i < 4; ++i) v[i] = fmaf(four[i], f, v[i]);
   };
-  // Statistics of up to 64 pieces, one in a lane, and the first rows of their sums: all loads at
-  // once. Calls of more pieces go on in turns of 64.
-  constexpr int kAhead = 4;
-  float m = kLowest, l = 0.0f, v[4] = {};
-  for (int turn = 0; turn < pieces.count; turn += kWave) {
-    const int here = min(pieces.count - turn, kWave);
-    const float2 st = lane < here ? a.part_stats[first + (turn + lane) * each] : float2{kLowest, 0.0f};
-    f32x4 ahead[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) ahead[i] = four_at(turn + share + i * shares);
-    float top = fmaxf(m, st.x);
-    for (int by = 32; by; by /= 2) top = fmaxf(top, __shfl_xor(top, by));
-    const float old = m == kLowest ? 0.0f : __builtin_amdgcn_exp2f((m - top) * unit);
-    const float mine = st.x == kLowest ? 0.0f : st.x == top ? 1.0f : __builtin_amdgcn_exp2f((st.x - top) * unit);
-    l *= old;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] *= old;
+  auto raise = [&](float top) __attribute__((always_inline)) {
+    const float f = m == kLowest ? 0.0f : __builtin_amdgcn_exp2f((m - top) * unit);
     m = top;
-    auto add = [&](int s, f32x4 four) __attribute__((always_inline)) {
-      const float f = __shfl(mine, s), sum = __shfl(st.y, s);
-      if (s >= here) return;
-      l = fmaf(sum, f, l);
+    l *= f;
+    v *= f;
+  };
+  constexpr int kAhead = 4;
+  for (int s = share; s < pieces.count; s += kAhead * shares) {
+    float2 st[kAhead];
+    f32x4 four[kAhead];
+    float top = m;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = fmaf(four[i], f, v[i]);
-    };
+    for (int i = 0; i < kAhead; ++i) {
+      const int piece = s + i * shares;
+      const bool here = live && piece < pieces.count;
+      const int64_t at = first + piece * each;
+      const float* p = a.part + at * a.D + d;
+      st[i] = here ? a.part_stats[at] : float2{kLowest, 0.0f};
+      four[i] = f32x4{0, 0, 0, 0};
+      if (here && left > 0) {
+        if (a.D % 4 == 0) {
+          four[i] = *reinterpret_cast<const f32x4*>(p);
+        } else {
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) add(share + i * shares, ahead[i]);
-    for (int s = kAhead * shares; s < here; s += shares) add(share + s, share + s < here ? four_at(turn + share + s) : f32x4{0, 0, 0, 0});
+          for (int j = 0; j < 4; ++j)
+            if (j < left) four[i][j] = p[j];
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) top = fmaxf(top, st[i].x);
+    raise(top);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) join(st[i], four[i], top);
   }
-  for (int by = lanes; by < kWave; by *= 2) {
-    l += __shfl_xor(l, by);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] += __shfl_xor(v[i], by);
+  if (shares > 1) {
+    sums[threadIdx.x] = v;
+    stats[threadIdx.x] = float2{m, l};
+    __syncthreads();
+    if (share > 0) return;
+    for (int i = 1; i < shares; ++i) {
+      const float2 st = stats[threadIdx.x + i * lanes];
+      raise(fmaxf(m, st.x));
+      join(st, sums[threadIdx.x + i * lanes], m);
+    }
   }
-  if (share > 0) return;
+  if (!live) return;
   const float inverse = m == kLowest ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] *= inverse;
-  const RowOf o = row_of(a, kv, uint32_t(row % a.R));
+  const float out_v[4] = {v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse};
+  const RowOf o = row_of(a, kv, uint32_t(r));
   T* out = static_cast<T*>(a.out) + ((int64_t(b) * a.Q + o.query) * (a.K * a.G) + o.head) * a.D;
-  store_four(out + d, v, left, a.out_vector);
+  store_four(out + d, out_v, left, a.out_vector);
   if (a.stats && lane == 0)
     a.stats[stat_at(a, b, o)] = m == kLowest ? float2{INFINITY, 0.0f} : float2{m, log2f(l) - kForwardBits<T>};
 }
@@ -887,9 +887,9 @@ __global__ __launch_bounds__(kThreads, grad_q_waves(sizeof(T), DP, MASK)) void a
     if (Shape::kBuffers == 1 && tile > w.first) __syncthreads();
     stage.k.store(k_tile);
     stage.v.store(v_tile);
-    MaskBytes mask[KB];
+    uint32_t mask[KB];
 #pragma unroll
-    for (int n = 0; n < KB; ++n) mask[n] = stage.next[n];
+    for (int n = 0; n < KB; ++n) mask[n] = MASK == kBoolMask ? stage.next[n] : 0;
     __syncthreads();
     if (tile + 1 < w.last) stage.load(tile + 1);
 
@@ -897,7 +897,8 @@ __global__ __launch_bounds__(kThreads, grad_q_waves(sizeof(T), DP, MASK)) void a
     for (int n = 0; n < KB; ++n) {
       const int here = local + 32 * n, key0 = tile * kKeys + here;
       if constexpr (MASK == kBoolMask)
-        if (!__any(mask[n].any() && live)) continue;
+        if (!__any(mask[n] != 0 && live)) continue;
+      const uint32_t bits = result_bits(mask[n]);
       float add[16];
       if constexpr (MASK == kFloatMask) float_masks(a, mask_at, key0, add);
       f32x16 s = {}, dp = {};
@@ -913,7 +914,7 @@ __global__ __launch_bounds__(kThreads, grad_q_waves(sizeof(T), DP, MASK)) void a
         const float y = MASK == kFloatMask ? fmaf(fmaf(s[i], factor, add[i]) - stat.x, kLog2e, shift)
                                            : fmaf(s[i], factor, shift);
         ds[i] = __builtin_amdgcn_exp2f(y) * fmaf(dp[i], scaled.power, -low);
-        if constexpr (MASK == kBoolMask) ds[i] = mask[n].on(i) ? ds[i] : 0.0f;
+        if constexpr (MASK == kBoolMask) ds[i] = where_bit(bits, 8 * (i / 4) + i % 4, ds[i], 0.0f);
         if constexpr (MASK == kFloatMask) ds[i] = add[i] == kLowest ? 0.0f : ds[i];
       }
       if (key0 + 32 > w.states) {
@@ -985,14 +986,6 @@ template <typename T, int DP> struct StatesShape {
   static constexpr int kLds = 2 * kBuffer;
 };
 
-// The non-zero bytes of four as four bits.
-__device__ inline uint32_t byte_bits(uint32_t four) {
-  uint32_t x = four | (four >> 4);
-  x |= x >> 2;
-  x |= x >> 1;
-  return (((x & 0x01010101u) * 0x01020408u) >> 24) & 15u;
-}
-
 template <typename T, int DP, int MASK>
 __global__ __launch_bounds__(kThreads, grad_states_waves(sizeof(T), DP, MASK)) void attention_grad_states_kernel(const Args a) {
   using Shape = StatesShape<T, DP>;
@@ -1020,7 +1013,7 @@ __global__ __launch_bounds__(kThreads, grad_states_waves(sizeof(T), DP, MASK)) v
   const bool words = MASK == kBoolMask && !a.mask_of_keys;
   bool on = key < states;
   if constexpr (MASK == kBoolMask)
-    if (a.mask_of_keys && on) on = bool_mask(a, b * a.mask_batch + int64_t(key) * a.mask_key);
+    if (a.mask_of_keys && on) on = state_bit(a, b, key);
 
   // Tiles of every head of the group in turn.
   const int query_tiles = (a.Q + kRows - 1) / kRows;
@@ -1034,7 +1027,7 @@ __global__ __launch_bounds__(kThreads, grad_states_waves(sizeof(T), DP, MASK)) v
   go_stage.plan(a.go.row, a.Dp);
   float2 stat = {INFINITY, 0.0f};
   float delta = 0.0f;
-  uint32_t raw[8];
+  uint32_t word = 0;
   int64_t float_at = 0, float_next = 0;  // the tile's first mask element, and its rows (float masks)
   int float_rows = 0, float_left = 0;
   auto load = [&]() __attribute__((always_inline)) {  // the next tile
@@ -1053,20 +1046,9 @@ __global__ __launch_bounds__(kThreads, grad_states_waves(sizeof(T), DP, MASK)) v
       float_left = left;
     }
     if (words && threadIdx.x < kRows * kWaves) {  // row threadIdx.x / 4, keys 32 (threadIdx.x % 4) ..
-      const int row = threadIdx.x / kWaves, k0 = key_tile * Shape::kKeys + 32 * int(threadIdx.x % kWaves);
+      const int row = threadIdx.x / kWaves;
       const int64_t at = mask_row_at(a, b, RowOf{query + (row < left ? row : left - 1), head});
-      const uint8_t* bytes = static_cast<const uint8_t*>(a.mask) + at;
-      if (k0 + 32 <= a.mask_row_keys) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const u32x4 four = load_anywhere<u32x4>(bytes + k0 + 16 * i);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) raw[4 * i + j] = four[j];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) raw[i] = four_bytes(a, bytes, k0 + 4 * i);
-      }
+      word = static_cast<const uint32_t*>(a.mask)[at + key_tile * (Shape::kKeys / 32) + int(threadIdx.x % kWaves)];
     }
     if (++next_tile == query_tiles) {
       next_tile = 0;
@@ -1105,12 +1087,8 @@ __global__ __launch_bounds__(kThreads, grad_states_waves(sizeof(T), DP, MASK)) v
       row_delta[threadIdx.x] = -delta;
       if constexpr (MASK == kFloatMask) row_max[threadIdx.x] = stat.x;
     }
-    if (words && threadIdx.x < kRows * kWaves) {
-      uint32_t word = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) word |= byte_bits(raw[i]) << (4 * i);
+    if (words && threadIdx.x < kRows * kWaves)
       row_words[(threadIdx.x % kWaves) * kRows + threadIdx.x / kWaves] = word;
-    }
     float_at = float_next;
     float_rows = float_left;
     __syncthreads();
@@ -1252,7 +1230,40 @@ __global__ __launch_bounds__(kThreads) void attention_sum_kernel(const Args a, i
   store_four(out + at, four, int(n - at < 4 ? n - at : 4), vector && reinterpret_cast<uintptr_t>(out) % 16 == 0);
 }
 
-// A mask whose keys do not lie side by side, or of fewer than 4, as rows of `keys` (a multiple
+// A bool mask's bytes as words of 32 keys, `words` of them for a row (a multiple of 4), one
+// thread each. The kernels read a row's mask several times (every head of a mask that is one for
+// all, forward and backward), as words at an eighth of the bytes, and two operations for each
+// score. Bound by the bytes read. Axes of stride 0 have size 1.
+inline __global__ __launch_bounds__(256) void attention_mask_bits_kernel(const uint8_t* from, uint32_t* to, int64_t batch,
+                                                                         int64_t head, int64_t row, int64_t key, int heads,
+                                                                         int rows, int S, int words, int64_t count) {
+  const int64_t n = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (n >= count) return;
+  const int word = int(n % words), k0 = 32 * word;
+  int64_t at = n / words;
+  const int64_t r = at % rows;
+  at /= rows;
+  const uint8_t* bytes = from + (at / heads) * batch + (at % heads) * head + r * row;
+  uint32_t bits = 0;
+  if (key == 1 && k0 + 32 <= S) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const u32x4 four = load_anywhere<u32x4>(bytes + k0 + 16 * i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t x = four[j] | (four[j] >> 4);  // non-zero bytes to their lowest bits
+        x |= x >> 2;
+        x |= x >> 1;
+        bits |= ((((x & 0x01010101u) * 0x01020408u) >> 24) & 15u) << (16 * i + 4 * j);
+      }
+    }
+  } else {
+    for (int i = 0; i < 32 && k0 + i < S; ++i) bits |= uint32_t(bytes[(k0 + i) * key] != 0) << i;
+  }
+  to[n] = bits;
+}
+
+// A float mask whose keys do not lie side by side, or of fewer than 4, as rows of `keys` (a multiple
 // of 32), with zeros past S: one thread for each element. Axes of stride 0 have size 1.
 template <typename V>
 __global__ __launch_bounds__(256) void attention_pack_mask_kernel(const V* from, V* to, int64_t batch, int64_t head,
@@ -1328,10 +1339,12 @@ template <typename T> void launch_forward(const Args& a, int mask_kind, bool few
     });
   });
   if (a.splits > 1) {
-    int lanes = 1;
+    int lanes = 1, shares = 1;
     while (4 * lanes < a.D) lanes *= 2;
-    attention_combine_kernel<T><<<uint32_t(ceil_div(int64_t(a.B) * a.K * a.R, kWaves)), kThreads, 0, s>>>(
-        a, lanes, mask_kind == kFloatMask, few_rows ? 128 : 64);
+    while (lanes * shares < kThreads && 4 * shares < a.splits) shares *= 2;
+    const int rows = kThreads / (lanes * shares);
+    attention_combine_kernel<T><<<dim3(uint32_t(ceil_div(a.R, rows)), uint32_t(a.B * a.K)), kThreads, 0, s>>>(
+        a, lanes, shares, mask_kind == kFloatMask, few_rows ? 128 : 64);
   }
 }
 

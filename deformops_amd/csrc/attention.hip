@@ -21,6 +21,9 @@ bool rows_as_they_are(const deformops_attention& c, const void* p, const int64_t
          (rows <= 1 || (strides[1] >= c.channels && strides[1] * size <= (int64_t(1) << 23)));
 }
 
+// Words of a bool mask's row: of whole tiles of 128 keys.
+int64_t mask_words(int64_t keys) { return ceil_div(keys, 128) * 4; }
+
 // Where one operand's packed copy lies in the workspace, if it has one.
 struct Packed {
   bool on;
@@ -46,9 +49,12 @@ Plan plan_of(const deformops_attention& c) {
   p.few_rows = R <= 64 && size * DP < 512;
   const int64_t rows = p.few_rows ? 32 : 128, keys = p.few_rows ? 128 : 64;
   const int64_t groups = BK * ceil_div(R, rows), tiles = ceil_div(c.keys, keys);
-  // Pieces of the key axis (of the rows, in the states' kernel) for as many workgroups as the
-  // card holds at once: one more would wait for a whole turn.
+  // Pieces of the key axis (of the rows, in the states' kernel) where there is not a workgroup
+  // for every CU, and then for as many as the card holds at once: one more would wait for a
+  // whole turn. With a workgroup on every CU, the join costs more than fuller CUs give (7 x
+  // 2,664 rows of 716 keys: 53 us in two pieces, 17 in one).
   auto pieces = [](int64_t groups, int waves, int64_t tiles) {
+    if (groups >= kCus) return 1;
     return int(std::max<int64_t>(1, std::min<int64_t>(kCus * waves / std::max<int64_t>(1, groups), tiles / 2)));
   };
   // The LDS of a workgroup whose waves share the rows (ForwardShape), in KB of a CU's 160.
@@ -74,9 +80,11 @@ Plan plan_of(const deformops_attention& c) {
   p.k = pack(rows_as_they_are(c, c.key, c.key_strides, c.keys), c.keys, c.key_heads);
   p.v = pack(rows_as_they_are(c, c.value, c.value_strides, c.keys), c.keys, c.key_heads);
   const int64_t (&m)[4] = c.mask_strides;
-  if (c.mask_kind != kNoMask && c.keys && (m[3] != 1 || c.keys < 4))
-    p.mask = Packed{true, take((m[0] ? c.batch : 1) * (m[1] ? c.heads : 1) * (m[2] ? c.queries : 1) *
-                               ceil_div(c.keys, 32) * 32 * (c.mask_kind == kBoolMask ? 1 : element_size(c.mask_dtype)))};
+  if (c.mask_kind != kNoMask && (c.mask_kind == kBoolMask || m[3] != 1 || c.keys < 4)) {
+    const int64_t rows = (m[0] ? c.batch : 1) * (m[1] ? c.heads : 1) * (m[2] ? c.queries : 1);
+    p.mask = Packed{true, take(c.mask_kind == kBoolMask ? rows * mask_words(c.keys) * 4
+                                                        : rows * ceil_div(c.keys, 32) * 32 * element_size(c.mask_dtype))};
+  }
   p.part_at = take(p.splits > 1 ? p.splits * BK * R * c.channels * 4 : 0);
   const int64_t shared = at;
   p.part_stats_at = take(p.splits > 1 ? p.splits * BK * R * 8 : 0);
@@ -140,30 +148,34 @@ Args args_of(const deformops_attention& c, const Plan& p, void* workspace, hipSt
   a.q = rows_of(c, c.query, c.query_strides, p.q, c.queries, c.heads, ws, s);
   a.k = rows_of(c, c.key, c.key_strides, p.k, c.keys, c.key_heads, ws, s);
   a.v = rows_of(c, c.value, c.value_strides, p.v, c.keys, c.key_heads, ws, s);
-  if (c.mask_kind != kNoMask && c.keys) {
+  if (c.mask_kind != kNoMask) {
     const int64_t (&m)[4] = c.mask_strides;
     a.mask = c.mask;
-    a.mask_batch = m[0]; a.mask_head = m[1]; a.mask_row = m[2]; a.mask_key = m[3];
+    a.mask_batch = m[0]; a.mask_head = m[1]; a.mask_row = m[2];
     a.mask_row_keys = int(c.keys);
     a.mask_type = c.mask_dtype;
     a.mask_of_keys = c.mask_kind == kBoolMask && (m[1] == 0 || c.heads == 1) && (m[2] == 0 || c.queries == 1);
     if (p.mask.on) {
-      const int64_t keys = ceil_div(c.keys, 32) * 32;
       const int64_t images = m[0] ? c.batch : 1, heads = m[1] ? c.heads : 1, rows = m[2] ? c.queries : 1;
-      const int64_t elements = images * heads * rows * keys;
-      a.mask = ws + p.mask.at;
-      a.mask_batch = m[0] ? heads * rows * keys : 0;
-      a.mask_head = m[1] ? rows * keys : 0;
-      a.mask_row = m[2] ? keys : 0;
-      a.mask_key = 1;
-      a.mask_row_keys = int(keys);
+      const int64_t each = c.mask_kind == kBoolMask ? mask_words(c.keys) : ceil_div(c.keys, 32) * 32;
+      const int64_t count = images * heads * rows * each;
+      char* to = ws + p.mask.at;
+      a.mask = to;
+      a.mask_batch = m[0] ? heads * rows * each : 0;
+      a.mask_head = m[1] ? rows * each : 0;
+      a.mask_row = m[2] ? each : 0;
+      a.mask_row_keys = int(each);
+      const uint32_t groups = uint32_t(ceil_div(count, 256));
       auto pack = [&](auto v) {
         using V = decltype(v);
-        attention_pack_mask_kernel<V><<<uint32_t(ceil_div(elements, 256)), 256, 0, s>>>(
-            static_cast<const V*>(c.mask), reinterpret_cast<V*>(ws + p.mask.at), m[0], m[1], m[2], m[3], int(heads), int(rows),
-            int(c.keys), int(keys), elements);
+        attention_pack_mask_kernel<V><<<groups, 256, 0, s>>>(static_cast<const V*>(c.mask), reinterpret_cast<V*>(to), m[0],
+                                                             m[1], m[2], m[3], int(heads), int(rows), int(c.keys),
+                                                             int(each), count);
       };
-      if (c.mask_kind == kBoolMask) pack(uint8_t());
+      if (c.mask_kind == kBoolMask)
+        attention_mask_bits_kernel<<<groups, 256, 0, s>>>(static_cast<const uint8_t*>(c.mask),
+                                                          reinterpret_cast<uint32_t*>(to), m[0], m[1], m[2], m[3],
+                                                          int(heads), int(rows), int(c.keys), int(each), count);
       else if (c.mask_dtype == MSDA_F32) pack(uint32_t());
       else pack(uint16_t());
     }
@@ -197,6 +209,13 @@ template <typename F> void with_type(int dtype, F f) {
   else f(bf16_t());
 }
 
+// A mask of no elements is not read, whatever its strides say: their zeros would look like axes
+// that one element serves.
+deformops_attention without_empty_mask(deformops_attention c) {
+  if (c.queries == 0 || c.keys == 0) c.mask_kind = kNoMask;
+  return c;
+}
+
 int too_many(int64_t groups) {
   return groups > (int64_t(1) << 31) - 1
              ? fail(MSDA_ERR_UNSUPPORTED, "cross attention: %lld workgroups pass a grid", static_cast<long long>(groups))
@@ -209,8 +228,9 @@ extern "C" {
 
 const char* deformops_last_error(void) { return g_error; }
 
-int deformops_cross_attention_workspace_size(const deformops_attention* c, int64_t* forward, int64_t* backward) {
-  if (const int e = check(c)) return e;
+int deformops_cross_attention_workspace_size(const deformops_attention* call, int64_t* forward, int64_t* backward) {
+  if (const int e = check(call)) return e;
+  const deformops_attention given = without_empty_mask(*call), *c = &given;
   if (!forward || !backward) return fail(MSDA_ERR_INVALID, "cross attention: null result");
   const Plan p = plan_of(*c);
   *forward = p.forward_bytes;
@@ -218,11 +238,12 @@ int deformops_cross_attention_workspace_size(const deformops_attention* c, int64
   return MSDA_OK;
 }
 
-int deformops_cross_attention_forward(const deformops_attention* c, void* row_stats, void* workspace,
+int deformops_cross_attention_forward(const deformops_attention* call, void* row_stats, void* workspace,
                                       int64_t workspace_bytes, void* stream) {
-  if (const int e = check(c)) return e;
+  if (const int e = check(call)) return e;
+  const deformops_attention given = without_empty_mask(*call), *c = &given;
   if (c->batch == 0 || c->queries == 0) return MSDA_OK;
-  if (!c->query || !c->output || (c->keys && (!c->key || !c->value)) || (c->keys && c->mask_kind && !c->mask))
+  if (!c->query || !c->output || (c->keys && (!c->key || !c->value)) || (c->mask_kind && !c->mask))
     return fail(MSDA_ERR_INVALID, "cross attention: null tensor");
   const Plan p = plan_of(*c);
   if (p.forward_bytes && (!workspace || workspace_bytes < p.forward_bytes || !aligned(workspace, 256)))
@@ -239,14 +260,15 @@ int deformops_cross_attention_forward(const deformops_attention* c, void* row_st
   return launched("cross attention forward");
 }
 
-int deformops_cross_attention_backward(const deformops_attention* c, const void* row_stats, const void* grad_output,
+int deformops_cross_attention_backward(const deformops_attention* call, const void* row_stats, const void* grad_output,
                                        void* grad_query, void* grad_key, void* grad_value, void* workspace,
                                        int64_t workspace_bytes, void* stream) {
-  if (const int e = check(c)) return e;
+  if (const int e = check(call)) return e;
+  const deformops_attention given = without_empty_mask(*call), *c = &given;
   if (c->batch == 0 || (c->queries == 0 && c->keys == 0)) return MSDA_OK;
   if ((c->queries && (!c->query || !c->output || !row_stats || !grad_output || !grad_query)) ||
       (c->keys && (!c->key || !c->value || !grad_key || !grad_value)) ||
-      (c->keys && c->queries && c->mask_kind && !c->mask))
+      (c->mask_kind && !c->mask))
     return fail(MSDA_ERR_INVALID, "cross attention: null tensor");
   const Plan p = plan_of(*c);
   if (p.backward_bytes && (!workspace || workspace_bytes < p.backward_bytes || !aligned(workspace, 256)))

@@ -276,7 +276,7 @@ def test_layouts(device, dtype):
 
 
 @pytest.mark.parametrize("device", BACKENDS)
-@pytest.mark.parametrize("sizes", [(0, 3, 4, 2, 2, 8), (2, 0, 4, 2, 1, 8), (2, 3, 0, 2, 1, 8), (1, 0, 0, 1, 1, 8)],
+@pytest.mark.parametrize("sizes", [(0, 3, 4, 2, 2, 8), (2, 0, 4, 2, 1, 8), (1, 0, 4, 1, 1, 8), (2, 3, 0, 2, 1, 8), (1, 0, 0, 1, 1, 8)],
                          ids=lambda s: "x".join(map(str, s)))
 @pytest.mark.parametrize("masked", [False, True])
 def test_empty_calls(device, sizes, masked):
