@@ -411,7 +411,8 @@ constexpr int forward_waves(int size, int DP, int mask) {
 constexpr int grad_q_waves(int size, int DP, int mask) {
   return size == 4 ? (DP > 32 ? 1 : 2) : DP == 32 ? 3 : DP <= (mask ? 64 : 96) ? 2 : 1;
 }
-constexpr int grad_states_waves(int size, int DP, int mask) {
+constexpr int grad_states_waves(int size, int DP, int mask, bool fused) {
+  if (fused && (DP == 32 || (DP == 64 && mask == kFloatMask))) return size == 4 || DP == 64 ? 1 : 2;
   return size == 4 ? (DP > 32 ? 1 : 2) : DP == 32 ? (mask ? 2 : 3) : DP == 64 ? 2 : 1;
 }
 
@@ -499,6 +500,32 @@ __device__ inline Pieces pieces_of(const Args& a, int b, int keys) {
   return Pieces{__builtin_amdgcn_readlane(s.before, b), __builtin_amdgcn_readlane(s.mine, b)};
 }
 
+// A wave's operand of 32 rows, straight from memory. By way of LDS, where neighbouring lanes would
+// read a row's neighbouring pieces, it was no faster for short calls and 3 % slower for long
+// ones (2 x 16,384 rows of 4,096 states: 1.37 and 1.39 ms, more registers).
+template <typename T, int DP>
+__device__ inline void take_rows(const Args& a, const T* row, bool live, u32x4 (&out)[Tile<T, DP>::kPieces / 2]) {
+#pragma unroll
+  for (int s = 0; s < Tile<T, DP>::kPieces / 2; ++s) {
+    const u32x4 zero = {0, 0, 0, 0};
+    out[s] = live ? load_piece(row, (2 * s + int(threadIdx.x % kWave) / 32) * (16 / int(sizeof(T))), a.Dp) : zero;
+  }
+}
+
+// A wave's channels x rows result, rounded to T, into the row of each lane (`image`: dense rows).
+template <typename T, int DP>
+__device__ __forceinline__ void write_row(const Args& a, T* image, RowOf o, const f32x16 (&acc)[DP / 32]) {
+  T* out = image + (int64_t(o.query) * (a.K * a.G) + o.head) * a.D;
+#pragma unroll
+  for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * c + 8 * g + 4 * (int(threadIdx.x % kWave) / 32);
+      const float v[4] = {acc[c][4 * g], acc[c][4 * g + 1], acc[c][4 * g + 2], acc[c][4 * g + 3]};
+      store_four(out + d, v, a.D - d, a.out_vector);
+    }
+}
+
 // What a workgroup of the walks over the keys works on. Row tiles of one piece of one key head
 // come first, then the heads: their rows share cache lines.
 template <typename Shape> struct KeyWalk {
@@ -539,12 +566,11 @@ template <typename T, int DP, int MASK, typename Shape> struct KeyStage {
   const KeyWalk<Shape>& w;
   Stage<T, DP, Shape::kKeys> k, v;
   const T *k_base, *v_base;
-  int64_t mask_at;
-  int local;  // this wave's first key in a tile
-  uint32_t next[KB];  // this row's mask words
+  int64_t mask_at = 0;  // this row's first mask element
+  int local;            // this wave's first key in a tile
+  uint32_t next[KB];    // this row's mask words
 
-  __device__ KeyStage(const Args& args, const KeyWalk<Shape>& walk, int64_t mask, int first_key)
-      : a(args), w(walk), mask_at(mask), local(first_key) {
+  __device__ KeyStage(const Args& args, const KeyWalk<Shape>& walk, int first_key) : a(args), w(walk), local(first_key) {
     k.plan(a.k.row, a.Dp);
     v.plan(a.v.row, a.Dp);
     k_base = static_cast<const T*>(a.k.at) + w.b * a.k.batch + w.kv * a.k.head;
@@ -563,10 +589,13 @@ template <typename T, int DP, int MASK, typename Shape> struct KeyStage {
       k.load(ks, left, All());
       v.load(vs, left, All());
     }
+    load_words(tile, next);
+  }
+  __device__ __forceinline__ void load_words(int tile, uint32_t (&words)[KB]) const {
     if constexpr (MASK == kBoolMask) {
 #pragma unroll
       for (int n = 0; n < KB; ++n)
-        next[n] = static_cast<const uint32_t*>(a.mask)[mask_at + (key + local) / 32 + n];
+        words[n] = static_cast<const uint32_t*>(a.mask)[mask_at + (tile * Shape::kKeys + local) / 32 + n];
     }
   }
 };
@@ -582,41 +611,24 @@ __global__ __launch_bounds__(kThreads, forward_waves(sizeof(T), DP, MASK)) void 
   const int wr = wave % WR, wk = wave / WR;
   const KeyWalk<Shape> w(a);
   if (w.b < 0) return;  // a slot that no image needs
+  const int local = 32 * KB * wk;
+  KeyStage<T, DP, MASK, Shape> stage(a, w, local);
+
   const uint32_t r = w.row_tile * Shape::kRows + 32 * wr + lane % 32;
   const bool live = r < a.R;
   const RowOf mine = row_of(a, w.kv, live ? r : a.R - 1);
-  int64_t mask_at = 0;
-  if constexpr (MASK != kNoMask) mask_at = mask_row_at(a, w.b, mine);
-  const int local = 32 * KB * wk;
-  KeyStage<T, DP, MASK, Shape> stage(a, w, mask_at, local);
+  if constexpr (MASK != kNoMask) stage.mask_at = mask_row_at(a, w.b, mine);
   if (w.first < w.last) stage.load(w.first);
-
   u32x4 q[kSteps];
-  {
-    const T* row = row_at<T>(a.q, w.b, mine);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const u32x4 zero = {0, 0, 0, 0};
-      q[s] = live ? load_piece(row, (2 * s + lane / 32) * (16 / int(sizeof(T))), a.Dp) : zero;
-    }
-  }
-
+  take_rows<T, DP>(a, row_at<T>(a.q, w.b, mine), live, q);
   Softmax<NB> soft;
+
   const float factor = MASK == kFloatMask ? a.scale : a.scale * kLog2e;
   constexpr float kStay = MASK == kFloatMask ? kSlack<T> / kLog2e : kSlack<T>;
 
-  auto step = [&](int tile, auto buffer) __attribute__((always_inline)) {
-    char* k_tile = lds + decltype(buffer)::value * 2 * Shape::kTile;
-    char* v_tile = k_tile + Shape::kTile;
-    if (Shape::kBuffers == 1 && tile > w.first) __syncthreads();
-    stage.k.store(k_tile);
-    stage.v.store(v_tile);
-    uint32_t mask[KB];
-#pragma unroll
-    for (int n = 0; n < KB; ++n) mask[n] = MASK == kBoolMask ? stage.next[n] : 0;
-    __syncthreads();
-    if (tile + 1 < w.last) stage.load(tile + 1);
-
+  auto attend = [&](int tile, auto buffer, const uint32_t (&mask)[KB]) __attribute__((always_inline)) {
+    const char* k_tile = lds + decltype(buffer)::value * 2 * Shape::kTile;
+    const char* v_tile = k_tile + Shape::kTile;
     const int key0 = tile * kKeys + local;  // this wave's keys
     if constexpr (MASK == kBoolMask) {
       uint32_t any = 0;
@@ -628,7 +640,7 @@ __global__ __launch_bounds__(kThreads, forward_waves(sizeof(T), DP, MASK)) void 
 #pragma unroll
     for (int n = 0; n < KB; ++n) {
       float add[16];
-      if constexpr (MASK == kFloatMask) float_masks(a, mask_at, key0 + 32 * n, add);
+      if constexpr (MASK == kFloatMask) float_masks(a, stage.mask_at, key0 + 32 * n, add);
       const uint32_t bits = result_bits(mask[n]);
       f32x16 s = {};
 #pragma unroll
@@ -677,6 +689,18 @@ __global__ __launch_bounds__(kThreads, forward_waves(sizeof(T), DP, MASK)) void 
     }
     soft.l += sum;
   };
+
+  auto step = [&](int tile, auto buffer) __attribute__((always_inline)) {
+    if (Shape::kBuffers == 1 && tile > w.first) __syncthreads();
+    stage.k.store(lds + decltype(buffer)::value * 2 * Shape::kTile);
+    stage.v.store(lds + decltype(buffer)::value * 2 * Shape::kTile + Shape::kTile);
+    uint32_t words[KB];
+#pragma unroll
+    for (int n = 0; n < KB; ++n) words[n] = MASK == kBoolMask ? stage.next[n] : 0;
+    __syncthreads();
+    if (tile + 1 < w.last) stage.load(tile + 1);
+    attend(tile, buffer, words);
+  };
   for (int tile = w.first; tile < w.last; tile += 2) {
     step(tile, Const<0>());
     if (tile + 1 < w.last) step(tile + 1, Const<Shape::kBuffers - 1>());
@@ -714,8 +738,8 @@ __global__ __launch_bounds__(kThreads, forward_waves(sizeof(T), DP, MASK)) void 
           soft.acc[c][i] = fmaf(at[(32 * c + result_row(i)) * 32 + lane % 32], f2, soft.acc[c][i]);
     }
   }
-  if (!live) return;
 
+  if (!live) return;
   if (a.splits > 1) {
     const int64_t at = w.part_row(a, r);
     if (lane < 32) a.part_stats[at] = float2{soft.m, soft.l};
@@ -734,17 +758,11 @@ __global__ __launch_bounds__(kThreads, forward_waves(sizeof(T), DP, MASK)) void 
   if (a.stats && lane < 32)
     a.stats[stat_at(a, w.b, mine)] = soft.m == kLowest ? float2{INFINITY, 0.0f}
                                                        : float2{soft.m, log2f(soft.l) - kForwardBits<T>};
-  T* out = static_cast<T*>(a.out) + ((int64_t(w.b) * a.Q + mine.query) * (a.K * a.G) + mine.head) * a.D;
 #pragma unroll
   for (int c = 0; c < NB; ++c)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = 32 * c + 8 * g + 4 * (lane / 32);
-      float v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = soft.acc[c][4 * g + i] * inverse;
-      store_four(out + d, v, a.D - d, a.out_vector);
-    }
+    for (int i = 0; i < 16; ++i) soft.acc[c][i] *= inverse;
+  write_row<T, DP>(a, static_cast<T*>(a.out) + w.b * (int64_t(a.Q) * (a.K * a.G) * a.D), mine, soft.acc);
 }
 
 // Joins the pieces of the forward's rows. A row has `lanes` lanes of four channels each, `shares`
@@ -851,28 +869,24 @@ __global__ __launch_bounds__(kThreads, grad_q_waves(sizeof(T), DP, MASK)) void a
   int64_t mask_at = 0;
   if constexpr (MASK != kNoMask) mask_at = mask_row_at(a, w.b, mine);
   const int local = 32 * KB * wk;
-  KeyStage<T, DP, MASK, Shape> stage(a, w, mask_at, local);
+  KeyStage<T, DP, MASK, Shape> stage(a, w, local);
+  stage.mask_at = mask_at;
   if (w.first < w.last) stage.load(w.first);
 
-  u32x4 q[kSteps], go[kSteps];
+  u32x4 q[kSteps], go[kSteps], o[kSteps];
+  take_rows<T, DP>(a, row_at<T>(a.q, w.b, mine), live, q);
+  take_rows<T, DP>(a, row_at<T>(a.go, w.b, mine), live, go);
+  take_rows<T, DP>(a, row_at<T>(a.o, w.b, mine), live, o);
   float delta = 0.0f;
-  {
-    const T *q_row = row_at<T>(a.q, w.b, mine), *go_row = row_at<T>(a.go, w.b, mine), *o_row = row_at<T>(a.o, w.b, mine);
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int c = (2 * s + lane / 32) * N;
-      const u32x4 zero = {0, 0, 0, 0};
-      q[s] = live ? load_piece(q_row, c, a.Dp) : zero;
-      go[s] = live ? load_piece(go_row, c, a.Dp) : zero;
-      const u32x4 o = live ? load_piece(o_row, c, a.Dp) : zero;
-      T x[N], y[N];
-      __builtin_memcpy(x, &go[s], 16);
-      __builtin_memcpy(y, &o, 16);
+  for (int s = 0; s < kSteps; ++s) {
+    T x[N], y[N];
+    __builtin_memcpy(x, &go[s], 16);
+    __builtin_memcpy(y, &o[s], 16);
 #pragma unroll
-      for (int i = 0; i < N; ++i) delta = fmaf(widen(x[i]), widen(y[i]), delta);
-    }
-    delta = half_sum(delta);
+    for (int i = 0; i < N; ++i) delta = fmaf(widen(x[i]), widen(y[i]), delta);
   }
+  delta = half_sum(delta);
   const float2 stat = live ? a.row_stats[stat_at(a, w.b, mine)] : float2{INFINITY, 0.0f};
   if (w.leads && wk == 0 && live && lane < 32) a.delta[stat_at(a, w.b, mine)] = delta;
 
@@ -954,20 +968,21 @@ __global__ __launch_bounds__(kThreads, grad_q_waves(sizeof(T), DP, MASK)) void a
         for (int i = 0; i < 16; ++i) acc[c][i] += at[(32 * c + result_row(i)) * 32 + lane % 32];
     }
   }
-  if (!live) return;
-  // A piece's sums lie in the order of an image's grad_q.
-  const int64_t in_image = (int64_t(mine.query) * (a.K * a.G) + mine.head) * a.D;
   const int64_t of_image = int64_t(a.Q) * (a.K * a.G) * a.D;
+  if (!live) return;
+  if (a.splits == 1) {
+    write_row<T, DP>(a, static_cast<T*>(a.grad_q) + w.b * of_image, mine, acc);
+    return;
+  }
+  // A piece's sums lie in the order of an image's grad_q.
+  float* part = a.part + w.slot * of_image + (int64_t(mine.query) * (a.K * a.G) + mine.head) * a.D;
 #pragma unroll
   for (int c = 0; c < NB; ++c)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int d = 32 * c + 8 * g + 4 * (lane / 32);
       const float v[4] = {acc[c][4 * g], acc[c][4 * g + 1], acc[c][4 * g + 2], acc[c][4 * g + 3]};
-      if (a.splits > 1)
-        store_four(a.part + w.slot * of_image + in_image + d, v, a.D - d, a.D % 4 == 0);
-      else
-        store_four(static_cast<T*>(a.grad_q) + w.b * of_image + in_image + d, v, a.D - d, a.out_vector);
+      store_four(part + d, v, a.D - d, a.D % 4 == 0);
     }
 }
 
@@ -984,15 +999,57 @@ template <typename T, int DP> struct StatesShape {
   static constexpr int kWords = kRows * kWaves * 4;  // a bool mask: 32 keys' bits for each row and wave
   static constexpr int kBuffer = 2 * kTile + kWords + kRows * 3 * 4;
   static constexpr int kLds = 2 * kBuffer;
+  // FUSED: the keys' tile and ds of a tile of rows.
+  static constexpr int kKeyTile = kKeys * Tile<T, DP>::kRowBytes;
+  static constexpr int kScoreTile = kRows * Tile<T, kKeys>::kRowBytes;
 };
 
-template <typename T, int DP, int MASK>
-__global__ __launch_bounds__(kThreads, grad_states_waves(sizeof(T), DP, MASK)) void attention_grad_states_kernel(const Args a) {
+// acc (channels x lanes) += tile^T (32 channels from 32 * block) x the rows' pieces `scores`, over
+// all kKeys tile rows in their order.
+template <typename T, int DP, int KEYS>
+__device__ inline f32x16 accumulate_rows(const char* tile, int block, const char* scores, int row, f32x16 acc) {
+  const int lane = threadIdx.x % kWave, half = lane / 32;
+#pragma unroll
+  for (int t = 0; t < Tile<T, KEYS>::kPieces / 2; ++t) {
+    const u32x4 b = row_piece<T, KEYS>(scores, row, t);
+    if constexpr (sizeof(T) == 2) {
+      const int channel = 32 * block + 16 * ((lane / 16) & 1) + 4 * (lane % 4);
+      i16x4 part[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int key = 16 * t + 8 * half + 4 * u + (lane % 16) / 4;
+        part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(
+            tile + Tile<T, DP>::offset(key, channel / 8) + (channel % 8) * 2));
+      }
+      const i16x8 both = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      acc = Mma<T>::mma(__builtin_bit_cast(typename Mma<T>::Vec, both), __builtin_bit_cast(typename Mma<T>::Vec, b), acc);
+    } else {
+      const int channel = 32 * block + lane % 32;
+      const f32x4 y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 8 * t + 4 * half + i;
+        const float x = *reinterpret_cast<const float*>(tile + Tile<T, DP>::offset(key, channel / 4) + (channel % 4) * 4);
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x, y[i], acc, 0, 0, 0);
+      }
+    }
+  }
+  return acc;
+}
+
+// FUSED: all states fill one workgroup's keys. Then it forms dq of its rows too, from ds in LDS,
+// and delta from the outputs: one pass over the rows' bytes, which bound calls of many rows and
+// few states, and 5 products in place of 7. Not in f16, whose ds has a scale for each key that a
+// sum over the keys cannot use.
+template <typename T, int DP, int MASK, bool FUSED>
+__global__ __launch_bounds__(kThreads, grad_states_waves(sizeof(T), DP, MASK, FUSED)) void attention_grad_states_kernel(const Args a) {
   using Shape = StatesShape<T, DP>;
   using TileT = Tile<T, DP>;
   constexpr int NB = DP / 32, kSteps = TileT::kPieces / 2, kRows = Shape::kRows;
   constexpr int N = 16 / int(sizeof(T));
-  __shared__ __attribute__((aligned(16))) char lds[Shape::kLds];
+  __shared__ __attribute__((aligned(16))) char lds[Shape::kLds + (FUSED ? Shape::kKeyTile + Shape::kScoreTile : 0)];
+  char* const key_rows = lds + Shape::kLds;  // FUSED
+  char* const scores = key_rows + Shape::kKeyTile;
 
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   // The heads whose rows share a cache line first (the key heads are a multiple of `near`),
@@ -1019,17 +1076,27 @@ __global__ __launch_bounds__(kThreads, grad_states_waves(sizeof(T), DP, MASK)) v
   const int query_tiles = (a.Q + kRows - 1) / kRows;
   const int64_t tiles = int64_t(query_tiles) * a.G;
   int64_t first = tiles * split / a.row_splits, last = tiles * (split + 1) / a.row_splits;
-  if (key_tile * Shape::kKeys >= states) last = first;  // padding only: zeros
+  // Padding only: zeros. FUSED goes on to write dq, which is 0 then.
+  if (!FUSED && key_tile * Shape::kKeys >= states) last = first;
   int next_head = int(first / (query_tiles ? query_tiles : 1)), next_tile = int(first - int64_t(next_head) * query_tiles);
 
-  Stage<T, DP, kRows> q_stage, go_stage;
+  Stage<T, DP, kRows> q_stage, go_stage, o_stage;
   q_stage.plan(a.q.row, a.Dp);
   go_stage.plan(a.go.row, a.Dp);
+  if constexpr (FUSED) {
+    o_stage.plan(a.o.row, a.Dp);
+    Stage<T, DP, Shape::kKeys> keys;
+    keys.plan(a.k.row, a.Dp);
+    auto kept = [&](int row) { return MASK != kBoolMask || !a.mask_of_keys || (row < states && state_bit(a, b, row)); };
+    keys.load(static_cast<const T*>(a.k.at) + b * a.k.batch + kv * a.k.head, states, kept);
+    keys.store(key_rows);
+  }
   float2 stat = {INFINITY, 0.0f};
   float delta = 0.0f;
   uint32_t word = 0;
   int64_t float_at = 0, float_next = 0;  // the tile's first mask element, and its rows (float masks)
   int float_rows = 0, float_left = 0;
+  int row_head = 0, row_query = 0, row_head_next = 0, row_query_next = 0;
   auto load = [&]() __attribute__((always_inline)) {  // the next tile
     const int head = kv * a.G + next_head, query = next_tile * kRows, left = a.Q - query;
     q_stage.load(static_cast<const T*>(a.q.at) + b * a.q.batch + head * a.q.head + int64_t(query) * a.q.row, left, All());
@@ -1039,8 +1106,12 @@ __global__ __launch_bounds__(kThreads, grad_states_waves(sizeof(T), DP, MASK)) v
       const bool live = int(threadIdx.x) < left;
       const int64_t at = (int64_t(b) * (a.K * a.G) + head) * a.Q + query + threadIdx.x;
       stat = live ? a.row_stats[at] : float2{INFINITY, 0.0f};
-      delta = live ? a.delta[at] : 0.0f;
+      if constexpr (!FUSED) delta = live ? a.delta[at] : 0.0f;
     }
+    if constexpr (FUSED)
+      o_stage.load(static_cast<const T*>(a.o.at) + b * a.o.batch + head * a.o.head + int64_t(query) * a.o.row, left, All());
+    row_head_next = head;
+    row_query_next = query;
     if constexpr (MASK == kFloatMask) {
       float_next = mask_row_at(a, b, RowOf{query, head});
       float_left = left;
@@ -1073,6 +1144,10 @@ __global__ __launch_bounds__(kThreads, grad_states_waves(sizeof(T), DP, MASK)) v
   f32x16 grad_k[NB] = {}, grad_v[NB] = {};
   Scaled<T> scaled;
   const float factor = MASK == kFloatMask ? a.scale : a.scale * kLog2e;
+  auto put_score = [&](int row, float v) __attribute__((always_inline)) {
+    const int at = 32 * wave + lane % 32;
+    *reinterpret_cast<T*>(scores + Tile<T, Shape::kKeys>::offset(row, at / N) + (at % N) * int(sizeof(T))) = static_cast<T>(v);
+  };
   auto step = [&](int64_t tile, auto buffer) __attribute__((always_inline)) {
     char* q_tile = lds + decltype(buffer)::value * Shape::kBuffer;
     char* go_tile = q_tile + Shape::kTile;
@@ -1084,13 +1159,29 @@ __global__ __launch_bounds__(kThreads, grad_states_waves(sizeof(T), DP, MASK)) v
     go_stage.store(go_tile);
     if (threadIdx.x < kRows) {
       row_shift[threadIdx.x] = kWeightBits<T> - (MASK == kFloatMask ? stat.y : stat.x + stat.y);
-      row_delta[threadIdx.x] = -delta;
+      if constexpr (!FUSED) row_delta[threadIdx.x] = -delta;
       if constexpr (MASK == kFloatMask) row_max[threadIdx.x] = stat.x;
+    }
+    if constexpr (FUSED) {  // the lanes of a row, a power of two, add up do . o
+#pragma unroll
+      for (int i = 0; i < Stage<T, DP, kRows>::kEach; ++i) {
+        T x[N], y[N];
+        __builtin_memcpy(x, &go_stage.hold[i], 16);
+        __builtin_memcpy(y, &o_stage.hold[i], 16);
+        float dot = 0.0f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) dot = fmaf(widen(x[j]), widen(y[j]), dot);
+#pragma unroll
+        for (int by = 1; by < TileT::kPieces; by *= 2) dot += __shfl_xor(dot, by);
+        if (o_stage.piece(i) == 0) row_delta[o_stage.row(i)] = -dot;
+      }
     }
     if (words && threadIdx.x < kRows * kWaves)
       row_words[(threadIdx.x % kWaves) * kRows + threadIdx.x / kWaves] = word;
     float_at = float_next;
     float_rows = float_left;
+    row_head = row_head_next;
+    row_query = row_query_next;
     __syncthreads();
     if (tile + 1 < last) load();
 
@@ -1107,7 +1198,13 @@ __global__ __launch_bounds__(kThreads, grad_states_waves(sizeof(T), DP, MASK)) v
 #pragma unroll
           for (int j = 0; j < 4; ++j) bits |= ((four[j] >> (lane % 32)) & 1) << (4 * g + j);
         }
-        if (!__any(on && bits != 0)) continue;
+        if (!__any(on && bits != 0)) {
+          if constexpr (FUSED) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) put_score(local + result_row(i), 0.0f);
+          }
+          continue;
+        }
       } else if constexpr (MASK == kFloatMask) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -1151,10 +1248,31 @@ __global__ __launch_bounds__(kThreads, grad_states_waves(sizeof(T), DP, MASK)) v
       const auto wp = Mma<T>::weights(p);
 #pragma unroll
       for (int c = 0; c < NB; ++c) grad_v[c] = accumulate<T, DP>(go_tile, local, c, wp, grad_v[c]);
+      if constexpr (FUSED) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) put_score(local + result_row(i), on ? ds[i] : 0.0f);
+      }
       scaled.fit(ds, grad_k);
       const auto ws = Mma<T>::weights(ds);
 #pragma unroll
       for (int c = 0; c < NB; ++c) grad_k[c] = accumulate<T, DP>(q_tile, local, c, ws, grad_k[c]);
+    }
+    if constexpr (FUSED) {  // dq: blocks of 32 rows x 32 channels, shared by the waves
+      __syncthreads();
+      for (int job = wave; job < Shape::RB * NB; job += kWaves) {
+        const int local = 32 * (job % Shape::RB), block = job / Shape::RB, query = row_query + local + lane % 32;
+        const f32x16 acc = accumulate_rows<T, DP, Shape::kKeys>(key_rows, block, scores, local, f32x16{});
+        if (query >= a.Q) continue;
+        T* to = static_cast<T*>(a.grad_q) + ((int64_t(b) * a.Q + query) * (a.K * a.G) + row_head) * a.D;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int d = 32 * block + 8 * g + 4 * (lane / 32);
+          float x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = acc[4 * g + i] * a.scale;
+          store_four(to + d, x, a.D - d, a.out_vector);
+        }
+      }
     }
   };
   for (int64_t tile = first; tile < last; tile += 2) {
@@ -1321,20 +1439,31 @@ template <typename F> void with_channels(int64_t D, F f) {
 }
 
 // `groups` and `key_groups`: workgroups of the walk over the keys and over the rows.
-template <typename T> void launch_forward(const Args& a, int mask_kind, bool few_rows, uint32_t groups, hipStream_t s);
+// Whether the states' kernel forms dq too where all keys fit its workgroup: not in f16 (its ds
+// has a scale for each key), not where a row's pieces are no power of two lanes (96 channels),
+// nor in f32 of 128 channels, which it would spill.
+constexpr bool fused_shape(bool f16, int size, int DP) { return !f16 && DP != 96 && DP * size < 512; }
+
+// What variant runs, by the plan of the call.
+struct Variant {
+  bool few_rows, fused;
+};
 template <typename T>
-void launch_backward(const Args& a, int mask_kind, bool few_rows, uint32_t groups, uint32_t key_groups, hipStream_t s);
+void launch_forward(const Args& a, int mask_kind, Variant variant, uint32_t groups, hipStream_t s);
+template <typename T>
+void launch_backward(const Args& a, int mask_kind, Variant variant, uint32_t groups, uint32_t key_groups, hipStream_t s);
 template <typename T>
 void launch_pack(const Rows& from, void* to, int64_t batch, int64_t rows, int heads, int D, int Dp, hipStream_t s);
 
 #ifdef ATTENTION_DEFINE_LAUNCHES
 
-template <typename T> void launch_forward(const Args& a, int mask_kind, bool few_rows, uint32_t groups, hipStream_t s) {
+template <typename T>
+void launch_forward(const Args& a, int mask_kind, Variant variant, uint32_t groups, hipStream_t s) {
   with_channels(a.D, [&](auto dp) {
     with_mask(mask_kind, [&](auto kind) {
       constexpr int DP = decltype(dp)::value, MASK = decltype(kind)::value;
       if constexpr (sizeof(T) * DP < 512)
-        if (few_rows) return attention_forward_kernel<T, DP, MASK, 1><<<groups, kThreads, 0, s>>>(a);
+        if (variant.few_rows) return attention_forward_kernel<T, DP, MASK, 1><<<groups, kThreads, 0, s>>>(a);
       attention_forward_kernel<T, DP, MASK, 4><<<groups, kThreads, 0, s>>>(a);
     });
   });
@@ -1344,29 +1473,31 @@ template <typename T> void launch_forward(const Args& a, int mask_kind, bool few
     while (lanes * shares < kThreads && 4 * shares < a.splits) shares *= 2;
     const int rows = kThreads / (lanes * shares);
     attention_combine_kernel<T><<<dim3(uint32_t(ceil_div(a.R, rows)), uint32_t(a.B * a.K)), kThreads, 0, s>>>(
-        a, lanes, shares, mask_kind == kFloatMask, few_rows ? 128 : 64);
+        a, lanes, shares, mask_kind == kFloatMask, variant.few_rows ? 128 : 64);
   }
 }
 
 template <typename T>
-void launch_backward(const Args& a, int mask_kind, bool few_rows, uint32_t groups, uint32_t key_groups, hipStream_t s) {
+void launch_backward(const Args& a, int mask_kind, Variant variant, uint32_t groups, uint32_t key_groups, hipStream_t s) {
   with_channels(a.D, [&](auto dp) {
     with_mask(mask_kind, [&](auto kind) {
       constexpr int DP = decltype(dp)::value, MASK = decltype(kind)::value;
+      if constexpr (fused_shape(std::is_same_v<T, f16_t>, sizeof(T), DP))
+        if (variant.fused) return attention_grad_states_kernel<T, DP, MASK, true><<<key_groups, kThreads, 0, s>>>(a);
       bool done = groups == 0;
       if constexpr (sizeof(T) * DP < 512)
-        if (few_rows && !done) {
+        if (variant.few_rows && !done) {
           attention_grad_q_kernel<T, DP, MASK, 1><<<groups, kThreads, 0, s>>>(a);
           done = true;
         }
       if (!done) attention_grad_q_kernel<T, DP, MASK, 4><<<groups, kThreads, 0, s>>>(a);
-      if (key_groups) attention_grad_states_kernel<T, DP, MASK><<<key_groups, kThreads, 0, s>>>(a);
+      if (key_groups) attention_grad_states_kernel<T, DP, MASK, false><<<key_groups, kThreads, 0, s>>>(a);
     });
   });
-  if (groups && a.splits > 1) {
+  if (groups && a.splits > 1 && !variant.fused) {
     const int64_t n = int64_t(a.Q) * a.K * a.G * a.D;
     attention_sum_kernel<T><<<dim3(uint32_t(ceil_div(n, 4 * kWave)), uint32_t(a.B)), kThreads, 0, s>>>(
-        a, n, few_rows ? 128 : 64);
+        a, n, variant.few_rows ? 128 : 64);
   }
   if (key_groups && a.row_splits > 1) {
     const int64_t n = int64_t(a.B) * a.S * a.K * a.D;
@@ -1383,8 +1514,8 @@ void launch_pack(const Rows& from, void* to, int64_t batch, int64_t rows, int he
 
 #define ATTENTION_INSTANTIATE(T)                                                                        \
   namespace attention {                                                                                 \
-  template void launch_forward<T>(const Args&, int, bool, uint32_t, hipStream_t);                       \
-  template void launch_backward<T>(const Args&, int, bool, uint32_t, uint32_t, hipStream_t);            \
+  template void launch_forward<T>(const Args&, int, Variant, uint32_t, hipStream_t);                    \
+  template void launch_backward<T>(const Args&, int, Variant, uint32_t, uint32_t, hipStream_t);         \
   template void launch_pack<T>(const Rows&, void*, int64_t, int64_t, int, int, int, hipStream_t);       \
   }
 

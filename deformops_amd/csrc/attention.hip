@@ -31,7 +31,7 @@ struct Packed {
 };
 
 struct Plan {
-  bool few_rows;   // one row tile of 32: the waves share the rows
+  Variant variant;  // few_rows: tiles of 32 rows, which the waves share
   int splits;      // of an image's keys
   bool balanced;   // splits by the images' lengths
   int row_splits;  // of the rows, in the states' kernel
@@ -46,25 +46,26 @@ Plan plan_of(const deformops_attention& c) {
   Plan p = {};
   const int64_t G = c.heads / c.key_heads, R = c.queries * G, BK = c.batch * c.key_heads;
   const int DP = padded(c.channels), size = element_size(c.dtype), n = 16 / size;
-  p.few_rows = R <= 64 && size * DP < 512;
-  const int64_t rows = p.few_rows ? 32 : 128, keys = p.few_rows ? 128 : 64;
+  p.variant.few_rows = R <= 64 && size * DP < 512;
+  const int64_t rows = p.variant.few_rows ? 32 : 128, keys = p.variant.few_rows ? 128 : 64;
   const int64_t groups = BK * ceil_div(R, rows), tiles = ceil_div(c.keys, keys);
   // Pieces of the key axis (of the rows, in the states' kernel) where there is not a workgroup
   // for every CU, and then for as many as the card holds at once: one more would wait for a
   // whole turn. With a workgroup on every CU, the join costs more than fuller CUs give (7 x
-  // 2,664 rows of 716 keys: 53 us in two pieces, 17 in one).
+  // 2,664 rows of 716 keys: 53 us in two pieces, 22 in one).
   auto pieces = [](int64_t groups, int waves, int64_t tiles) {
     if (groups >= kCus) return 1;
     return int(std::max<int64_t>(1, std::min<int64_t>(kCus * waves / std::max<int64_t>(1, groups), tiles / 2)));
   };
   // The LDS of a workgroup whose waves share the rows (ForwardShape), in KB of a CU's 160.
   const int tile = DP * size / 8, lds = 4 * tile <= 80 ? 4 * tile : std::max(2 * tile, DP / 2 + 1);
-  const int lds_waves = p.few_rows ? 160 / lds : 4;
+  const int lds_waves = p.variant.few_rows ? 160 / lds : 4;
   p.splits = pieces(groups, std::min(lds_waves, forward_waves(size, DP, c.mask_kind)), tiles);
+  p.variant.fused = c.keys > 0 && c.keys <= 128 && fused_shape(c.dtype == MSDA_F16, size, DP);
   p.balanced = p.splits > 1 && c.key_lengths && c.batch > 1 && c.batch <= 64;
   const int64_t row_tile = DP * size <= 192 ? 64 : 32;
   const int64_t key_groups = BK * ceil_div(c.keys, 128), row_tiles = G * ceil_div(c.queries, row_tile);
-  p.row_splits = pieces(key_groups, grad_states_waves(size, DP, c.mask_kind), row_tiles);
+  p.row_splits = pieces(key_groups, grad_states_waves(size, DP, c.mask_kind, p.variant.fused), row_tiles);
 
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -85,6 +86,7 @@ Plan plan_of(const deformops_attention& c) {
     p.mask = Packed{true, take(c.mask_kind == kBoolMask ? rows * mask_words(c.keys) * 4
                                                         : rows * ceil_div(c.keys, 32) * 32 * element_size(c.mask_dtype))};
   }
+  // (The backward's sums of grad_q; none of them where that is fused.)
   p.part_at = take(p.splits > 1 ? p.splits * BK * R * c.channels * 4 : 0);
   const int64_t shared = at;
   p.part_stats_at = take(p.splits > 1 ? p.splits * BK * R * 8 : 0);
@@ -253,10 +255,9 @@ int deformops_cross_attention_forward(const deformops_attention* call, void* row
   Args a = args_of(*c, p, workspace, s);
   a.stats = static_cast<float2*>(row_stats);
   a.out_vector = a.D % 4 == 0 && aligned(c->output, 16);
-  const int64_t rows = p.few_rows ? 32 : 128;
-  const int64_t groups = int64_t(a.B) * a.K * ceil_div(a.R, rows) * a.splits;
+  const int64_t groups = int64_t(a.B) * a.K * ceil_div(a.R, p.variant.few_rows ? 32 : 128) * a.splits;
   if (const int e = too_many(groups)) return e;
-  with_type(c->dtype, [&](auto t) { launch_forward<decltype(t)>(a, c->mask_kind, p.few_rows, uint32_t(groups), s); });
+  with_type(c->dtype, [&](auto t) { launch_forward<decltype(t)>(a, c->mask_kind, p.variant, uint32_t(groups), s); });
   return launched("cross attention forward");
 }
 
@@ -287,12 +288,11 @@ int deformops_cross_attention_backward(const deformops_attention* call, const vo
   a.grad_k = grad_key;
   a.grad_v = grad_value;
   a.out_vector = a.D % n == 0 && aligned(grad_query, 16) && aligned(grad_key, 16) && aligned(grad_value, 16);
-  const int64_t rows = p.few_rows ? 32 : 128;
-  const int64_t groups = int64_t(a.B) * a.K * ceil_div(a.R, rows) * a.splits;
+  const int64_t groups = int64_t(a.B) * a.K * ceil_div(a.R, p.variant.few_rows ? 32 : 128) * a.splits;
   const int64_t key_groups = int64_t(a.B) * a.K * ceil_div(a.S, 128) * a.row_splits;
   if (const int e = too_many(std::max(groups, key_groups))) return e;
   with_type(c->dtype, [&](auto t) {
-    launch_backward<decltype(t)>(a, c->mask_kind, p.few_rows, uint32_t(groups), uint32_t(key_groups), s);
+    launch_backward<decltype(t)>(a, c->mask_kind, p.variant, uint32_t(groups), uint32_t(key_groups), s);
   });
   return launched("cross attention backward");
 }
