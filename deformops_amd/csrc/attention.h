@@ -14,7 +14,7 @@
 // for the whole group, a group's gradients of k and v are summed in one place, and a single
 // token's G heads fill one tile.
 //
-// Products. All run on v_mfma_f32_32x32x16_{bf16,f16} or v_mfma_f32_32x32x2_f32, whose result
+// Products. All run on v_mfma_f32_32x32x16_{bf16,f16} (float as three bf16 parts), whose result
 // has column = lane % 32 and rows 8 (r / 4) + 4 (lane / 32) + r % 4 in its 16 registers. The
 // scores are formed so that the axis of the next product's contraction lies in the registers:
 // keys x rows for o and dq, rows x keys for dv and dk. A product contracts over its axis in
@@ -111,7 +111,9 @@ template <typename T> struct Mma;
 
 template <typename T> struct Mma16 {
   using Vec = std::conditional_t<std::is_same_v<T, bf16_t>, bf16x8, f16x8>;
-  struct Weights { Vec part[2]; };  // 32 contracted positions
+  static constexpr int kPlanes = 1;
+  struct Piece { u32x4 plane[1]; };          // 8 channels of a row
+  struct Weights { Vec part[2][1]; };        // 32 contracted positions
 
   static __device__ f32x16 mma(Vec a, Vec b, f32x16 c) {
     if constexpr (std::is_same_v<T, bf16_t>)
@@ -119,97 +121,148 @@ template <typename T> struct Mma16 {
     else
       return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
-  // One 16-byte piece of 32 rows of each operand: 16 contracted channels.
-  static __device__ f32x16 rows(u32x4 a, u32x4 b, f32x16 c) {
-    return mma(__builtin_bit_cast(Vec, a), __builtin_bit_cast(Vec, b), c);
-  }
+  static __device__ f32x16 product(const Vec (&a)[1], const Vec (&b)[1], f32x16 c) { return mma(a[0], b[0], c); }
   static __device__ Weights weights(const float (&w)[16]) {
     Weights out;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) out.part[i / 8][i % 8] = static_cast<T>(w[i]);
+    for (int i = 0; i < 16; ++i) out.part[i / 8][0][i % 8] = static_cast<T>(w[i]);
     return out;
   }
+  // 8 channels, 16 bytes, as an operand.
+  static __device__ Piece piece(const u32x4 (&memory)[1]) { return Piece{{memory[0]}}; }
 };
 template <> struct Mma<bf16_t> : Mma16<bf16_t> {};
 template <> struct Mma<f16_t> : Mma16<f16_t> {};
+
+// float on the bf16 matrix cores: x = x0 + x1 + x2 exactly, each part the rest rounded to bf16
+// (8 bits; the parts of a number below 2^-110 lose their last bits to bf16's range), and a product
+// is the sum of the six largest of the nine: what is left out, a1 b2 + a2 b1 + a2 b2, is at most
+// 2^-23 of it, float's own rounding. Six products of 32 cycles for 16 contracted channels, where
+// v_mfma_f32_32x32x2_f32 takes eight of 64 cycles (4 x 1,501 rows of 2,333 states, 8 heads of
+// 64, forward and backward: 1.40 ms with it, 0.90 with these). An infinite operand gives NaN.
 template <> struct Mma<float> {
-  struct Weights { float part[16]; };
-  static __device__ f32x16 rows(u32x4 a, u32x4 b, f32x16 c) {
-    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[i], c, 0, 0, 0);
-    return c;
+  using Vec = bf16x8;
+  static constexpr int kPlanes = 3;
+  struct Piece { u32x4 plane[3]; };
+  struct Weights { Vec part[2][3]; };
+
+  static __device__ void split(float x, bf16_t (&out)[3]) {
+    out[0] = static_cast<bf16_t>(x);
+    const float rest = x - static_cast<float>(out[0]);
+    out[1] = static_cast<bf16_t>(rest);
+    out[2] = static_cast<bf16_t>(rest - static_cast<float>(out[1]));
+  }
+  static __device__ f32x16 product(const Vec (&a)[3], const Vec (&b)[3], f32x16 c) {
+    c = Mma<bf16_t>::mma(a[2], b[0], c);  // the smallest first
+    c = Mma<bf16_t>::mma(a[0], b[2], c);
+    c = Mma<bf16_t>::mma(a[1], b[1], c);
+    c = Mma<bf16_t>::mma(a[1], b[0], c);
+    c = Mma<bf16_t>::mma(a[0], b[1], c);
+    return Mma<bf16_t>::mma(a[0], b[0], c);
   }
   static __device__ Weights weights(const float (&w)[16]) {
     Weights out;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) out.part[i] = w[i];
+    for (int i = 0; i < 16; ++i) {
+      bf16_t parts[3];
+      split(w[i], parts);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) out.part[i / 8][p][i % 8] = parts[p];
+    }
     return out;
+  }
+  static __device__ Piece piece(const u32x4 (&memory)[2]) {
+    Vec out[3];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      bf16_t parts[3];
+      split(__builtin_bit_cast(f32x4, memory[i / 4])[i % 4], parts);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) out[p][i] = parts[p];
+    }
+    return Piece{{__builtin_bit_cast(u32x4, out[0]), __builtin_bit_cast(u32x4, out[1]), __builtin_bit_cast(u32x4, out[2])}};
   }
 };
 
-// A tile of rows in LDS, DP channels each, in 16-byte pieces that change places within their row
-// by an exclusive or with bits of the row's number. LDS serves 64 banks (256 bytes) a cycle: 16
-// lanes of a row operand's read (one piece of 16 rows), or 32 lanes of a turning read (4
-// neighbouring pieces of 4 rows, 8 bytes a lane), have to lie in different sixteenths of 256
-// bytes. Measured on reads of both kinds: 540 and 300-320 bytes/ns a CU with these patterns,
-// 300 and 150 with `row & 7`.
-template <typename T, int DP> struct Tile {
-  static constexpr int kPieces = DP * int(sizeof(T)) / 16;
-  static constexpr int kRowBytes = kPieces * 16;
+// c += the rows' products over one piece of each: 16 contracted channels, 8 in each half of the
+// wave.
+template <typename T>
+__device__ inline f32x16 multiply(const typename Mma<T>::Piece& a, const typename Mma<T>::Piece& b, f32x16 c) {
+  typename Mma<T>::Vec x[Mma<T>::kPlanes], y[Mma<T>::kPlanes];
+#pragma unroll
+  for (int p = 0; p < Mma<T>::kPlanes; ++p) {
+    x[p] = __builtin_bit_cast(typename Mma<T>::Vec, a.plane[p]);
+    y[p] = __builtin_bit_cast(typename Mma<T>::Vec, b.plane[p]);
+  }
+  return Mma<T>::product(x, y, c);
+}
 
-  static __device__ int offset(int row, int piece) {
+// A tile of rows in LDS, DP channels each, as 16-bit elements (float: the three planes of a row
+// side by side) in 16-byte pieces that change places within their plane by an exclusive or with
+// bits of the row's number. LDS serves 64 banks (256 bytes) a cycle: 16 lanes of a row operand's
+// read (one piece of 16 rows), or 32 lanes of a turning read (4 neighbouring pieces of 4 rows, 8
+// bytes a lane), have to lie in different sixteenths of 256 bytes. Measured on reads of both
+// kinds: 540 and 300-320 bytes/ns a CU with these patterns, 300 and 150 with `row & 7`. (A row of
+// three planes is 12, 8, 4 or 0 sixteenths past a multiple of 256 bytes for 32, 64, 96 and 128
+// channels, as 192, 128, 64 and 256 bytes are, so the patterns serve it too.)
+template <typename T, int DP> struct Tile {
+  static constexpr int kPlanes = Mma<T>::kPlanes;
+  static constexpr int kPieces = DP / 8;  // of a plane
+  static constexpr int kRowBytes = kPlanes * DP * 2;
+
+  static __device__ int offset(int row, int piece, int plane = 0) {
     int turn;
-    if constexpr (sizeof(T) == 4)  // single channels of rows r and r + 4 are read together
-      turn = kPieces % 16 == 0 ? (row & 3) | ((row & 4) << 1) | ((row & 8) >> 1) : row & 7;
-    else if constexpr (kPieces == 16)
+    if constexpr (kPieces == 16)
       turn = ((row & 3) << 2) | ((row >> 2) & 3);
     else if constexpr (kPieces == 8)
       turn = ((row & 2) << 1) | ((row >> 2) & 3);
     else  // 4 or 12: rows r .. r + 3 differ in their sixteenths already
       turn = (row >> 2) & 3;
-    return row * kRowBytes + ((piece ^ turn) << 4);
+    return row * kRowBytes + plane * (DP * 2) + ((piece ^ turn) << 4);
   }
 };
+
+// The turning read of a tile: 8 contracted rows from `row0` and `row1` (4 each) of 32 channels.
+template <typename T, int DP>
+__device__ inline void turned(const char* tile, int row0, int row1, int block, typename Mma<T>::Vec (&out)[Mma<T>::kPlanes]) {
+  const int lane = threadIdx.x % kWave;
+  // Lane c of a 16-lane group gets channel c of the four rows that the group reads.
+  const int channel = 32 * block + 16 * ((lane / 16) & 1) + 4 * (lane % 4), within = (lane % 16) / 4;
+#pragma unroll
+  for (int p = 0; p < Mma<T>::kPlanes; ++p) {
+    i16x4 part[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(
+          tile + Tile<T, DP>::offset((u ? row1 : row0) + within, channel / 8, p) + (channel % 8) * 2));
+    out[p] = __builtin_bit_cast(typename Mma<T>::Vec, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+}
 
 // acc (channels x lanes) += tile^T (32 channels from 32 * block, the 32 tile rows from `row`)
 // x w: the sum over tile rows of w[row][lane] * tile[row][channel].
 template <typename T, int DP>
 __device__ inline f32x16 accumulate(const char* tile, int row, int block, const typename Mma<T>::Weights& w,
                                     f32x16 acc) {
-  const int lane = threadIdx.x % kWave, half = lane / 32;
-  if constexpr (sizeof(T) == 2) {
-    // Lane c of a 16-lane group gets channel c of the four rows that the group reads.
-    const int channel = 32 * block + 16 * ((lane / 16) & 1) + 4 * (lane % 4);
+  const int half = int(threadIdx.x % kWave) / 32;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      i16x4 part[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int r = row + 16 * t + 8 * u + 4 * half + (lane % 16) / 4;
-        const char* at = tile + Tile<T, DP>::offset(r, channel / 8) + (channel % 8) * 2;
-        part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) i16x4*)(at));
-      }
-      const i16x8 both = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
-      acc = Mma<T>::mma(__builtin_bit_cast(typename Mma<T>::Vec, both), w.part[t], acc);
-    }
-  } else {
-    const int channel = 32 * block + lane % 32;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int r = row + 8 * (i / 4) + 4 * half + i % 4;
-      const float a = *reinterpret_cast<const float*>(tile + Tile<T, DP>::offset(r, channel / 4) + (channel % 4) * 4);
-      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a, w.part[i], acc, 0, 0, 0);
-    }
+  for (int t = 0; t < 2; ++t) {
+    typename Mma<T>::Vec a[Mma<T>::kPlanes];
+    const int r = row + 16 * t + 4 * half;
+    turned<T, DP>(tile, r, r + 8, block, a);
+    acc = Mma<T>::product(a, w.part[t], acc);
   }
   return acc;
 }
 
 // The product's row operand: piece 2 * step + half of tile row `row + lane % 32`.
-template <typename T, int DP> __device__ inline u32x4 row_piece(const char* tile, int row, int step) {
+template <typename T, int DP> __device__ inline typename Mma<T>::Piece row_piece(const char* tile, int row, int step) {
   const int lane = threadIdx.x % kWave;
-  return *reinterpret_cast<const u32x4*>(tile + Tile<T, DP>::offset(row + lane % 32, 2 * step + lane / 32));
+  typename Mma<T>::Piece out;
+#pragma unroll
+  for (int p = 0; p < Mma<T>::kPlanes; ++p)
+    out.plane[p] = *reinterpret_cast<const u32x4*>(tile + Tile<T, DP>::offset(row + lane % 32, 2 * step + lane / 32, p));
+  return out;
 }
 
 // 16 bytes of a row in memory, from channel c; zero past Dp.
@@ -369,7 +422,7 @@ template <typename T> __device__ inline const T* uniform(const T* p) {
 }
 
 template <typename T, int DP, int ROWS> struct Stage {
-  static constexpr int kPieces = Tile<T, DP>::kPieces;
+  static constexpr int kPieces = DP * int(sizeof(T)) / 16;
   static constexpr int kEach = ROWS * kPieces / kThreads;
   static_assert(ROWS * kPieces % kThreads == 0);
   u32x4 hold[kEach];
@@ -396,7 +449,22 @@ template <typename T, int DP, int ROWS> struct Stage {
   }
   __device__ __forceinline__ void store(char* tile) const {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) *reinterpret_cast<u32x4*>(tile + Tile<T, DP>::offset(row(i), piece(i))) = hold[i];
+    for (int i = 0; i < kEach; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<u32x4*>(tile + Tile<T, DP>::offset(row(i), piece(i))) = hold[i];
+      } else {  // half a piece of each plane
+        bf16_t parts[4][3];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) Mma<T>::split(__builtin_bit_cast(f32x4, hold[i])[j], parts[j]);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+          const bf16_t four[4] = {parts[0][p], parts[1][p], parts[2][p], parts[3][p]};
+          u32x2 w;
+          __builtin_memcpy(&w, four, 8);
+          *reinterpret_cast<u32x2*>(tile + Tile<T, DP>::offset(row(i), piece(i) / 2, p) + 8 * (piece(i) % 2)) = w;
+        }
+      }
+    }
   }
 };
 
@@ -412,8 +480,8 @@ constexpr int grad_q_waves(int size, int DP, int mask) {
   return size == 4 ? (DP > 32 ? 1 : 2) : DP == 32 ? 3 : DP <= (mask ? 64 : 96) ? 2 : 1;
 }
 constexpr int grad_states_waves(int size, int DP, int mask, bool fused) {
-  if (fused && (DP == 32 || (DP == 64 && mask == kFloatMask))) return size == 4 || DP == 64 ? 1 : 2;
-  return size == 4 ? (DP > 32 ? 1 : 2) : DP == 32 ? (mask ? 2 : 3) : DP == 64 ? 2 : 1;
+  if (fused && (size == 4 || (DP == 64 && mask == kFloatMask))) return 1;
+  return size == 4 ? (DP > 32 ? 1 : 2) : DP == 32 ? (fused && mask ? 2 : 3) : DP == 64 ? 2 : 1;
 }
 
 // ---------------------------------------------------------------------------
@@ -427,7 +495,7 @@ template <typename T, int DP, int WR> struct ForwardShape {
   static constexpr int kRows = 32 * WR;
   static constexpr int kKeys = 32 * KB * WK;
   static constexpr int kTile = kKeys * Tile<T, DP>::kRowBytes;
-  static constexpr int kBuffers = 4 * kTile <= (forward_waves(sizeof(T), DP, kNoMask) > 1 ? 80 : 128) * 1024 ? 2 : 1;
+  static constexpr int kBuffers = 4 * kTile <= (forward_waves(sizeof(T), DP, kNoMask) > 1 ? 80 : 160) * 1024 ? 2 : 1;
   static constexpr int kJoin = WK > 1 ? WK * 32 * WR * (DP + 2) * 4 : 0;
   static constexpr int kLds = std::max(2 * kBuffers * kTile, kJoin);
 };
@@ -504,12 +572,35 @@ __device__ inline Pieces pieces_of(const Args& a, int b, int keys) {
 // read a row's neighbouring pieces, it was no faster for short calls and 3 % slower for long
 // ones (2 x 16,384 rows of 4,096 states: 1.37 and 1.39 ms, more registers).
 template <typename T, int DP>
-__device__ inline void take_rows(const Args& a, const T* row, bool live, u32x4 (&out)[Tile<T, DP>::kPieces / 2]) {
+__device__ inline void take_rows(const Args& a, const T* row, bool live, typename Mma<T>::Piece (&out)[DP / 16]) {
+  constexpr int N = 16 / int(sizeof(T)), kOfPiece = 8 / N;
 #pragma unroll
-  for (int s = 0; s < Tile<T, DP>::kPieces / 2; ++s) {
-    const u32x4 zero = {0, 0, 0, 0};
-    out[s] = live ? load_piece(row, (2 * s + int(threadIdx.x % kWave) / 32) * (16 / int(sizeof(T))), a.Dp) : zero;
+  for (int s = 0; s < DP / 16; ++s) {
+    u32x4 memory[kOfPiece];
+#pragma unroll
+    for (int i = 0; i < kOfPiece; ++i) {
+      const u32x4 zero = {0, 0, 0, 0};
+      memory[i] = live ? load_piece(row, (2 * s + int(threadIdx.x % kWave) / 32) * 8 + i * N, a.Dp) : zero;
+    }
+    out[s] = Mma<T>::piece(memory);
   }
+}
+
+// The sum of the products of two rows' channels, by the two lanes of the row.
+template <typename T, int DP> __device__ inline float row_dot(const Args& a, const T* x, const T* y) {
+  constexpr int N = 16 / int(sizeof(T));
+  float sum = 0.0f;
+#pragma unroll
+  for (int c = 0; c < DP; c += 2 * N) {
+    const int at = c + N * (int(threadIdx.x % kWave) / 32);
+    const u32x4 p = load_piece(x, at, a.Dp), q = load_piece(y, at, a.Dp);
+    T u[N], v[N];
+    __builtin_memcpy(u, &p, 16);
+    __builtin_memcpy(v, &q, 16);
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum = fmaf(widen(u[i]), widen(v[i]), sum);
+  }
+  return half_sum(sum);
 }
 
 // A wave's channels x rows result, rounded to T, into the row of each lane (`image`: dense rows).
@@ -619,7 +710,7 @@ __global__ __launch_bounds__(kThreads, forward_waves(sizeof(T), DP, MASK)) void 
   const RowOf mine = row_of(a, w.kv, live ? r : a.R - 1);
   if constexpr (MASK != kNoMask) stage.mask_at = mask_row_at(a, w.b, mine);
   if (w.first < w.last) stage.load(w.first);
-  u32x4 q[kSteps];
+  typename Mma<T>::Piece q[kSteps];
   take_rows<T, DP>(a, row_at<T>(a.q, w.b, mine), live, q);
   Softmax<NB> soft;
 
@@ -644,7 +735,7 @@ __global__ __launch_bounds__(kThreads, forward_waves(sizeof(T), DP, MASK)) void 
       const uint32_t bits = result_bits(mask[n]);
       f32x16 s = {};
 #pragma unroll
-      for (int t = 0; t < kSteps; ++t) s = Mma<T>::rows(row_piece<T, DP>(k_tile, local + 32 * n, t), q[t], s);
+      for (int t = 0; t < kSteps; ++t) s = multiply<T>(row_piece<T, DP>(k_tile, local + 32 * n, t), q[t], s);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         x[n][i] = s[i];
@@ -856,7 +947,6 @@ __global__ __launch_bounds__(kThreads, grad_q_waves(sizeof(T), DP, MASK)) void a
   using Shape = ForwardShape<T, DP, WR>;
   using TileT = Tile<T, DP>;
   constexpr int KB = Shape::KB, NB = DP / 32, kSteps = TileT::kPieces / 2, kKeys = Shape::kKeys;
-  constexpr int N = 16 / int(sizeof(T));
   __shared__ __attribute__((aligned(16))) char lds[Shape::kLds];
 
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
@@ -873,20 +963,11 @@ __global__ __launch_bounds__(kThreads, grad_q_waves(sizeof(T), DP, MASK)) void a
   stage.mask_at = mask_at;
   if (w.first < w.last) stage.load(w.first);
 
-  u32x4 q[kSteps], go[kSteps], o[kSteps];
+  typename Mma<T>::Piece q[kSteps], go[kSteps];
   take_rows<T, DP>(a, row_at<T>(a.q, w.b, mine), live, q);
   take_rows<T, DP>(a, row_at<T>(a.go, w.b, mine), live, go);
-  take_rows<T, DP>(a, row_at<T>(a.o, w.b, mine), live, o);
-  float delta = 0.0f;
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    T x[N], y[N];
-    __builtin_memcpy(x, &go[s], 16);
-    __builtin_memcpy(y, &o[s], 16);
-#pragma unroll
-    for (int i = 0; i < N; ++i) delta = fmaf(widen(x[i]), widen(y[i]), delta);
-  }
-  delta = half_sum(delta);
+  // Lanes past the last row repeat it.
+  const float delta = row_dot<T, DP>(a, row_at<T>(a.go, w.b, mine), row_at<T>(a.o, w.b, mine));
   const float2 stat = live ? a.row_stats[stat_at(a, w.b, mine)] : float2{INFINITY, 0.0f};
   if (w.leads && wk == 0 && live && lane < 32) a.delta[stat_at(a, w.b, mine)] = delta;
 
@@ -918,8 +999,8 @@ __global__ __launch_bounds__(kThreads, grad_q_waves(sizeof(T), DP, MASK)) void a
       f32x16 s = {}, dp = {};
 #pragma unroll
       for (int t = 0; t < kSteps; ++t) {
-        s = Mma<T>::rows(row_piece<T, DP>(k_tile, here, t), q[t], s);
-        dp = Mma<T>::rows(row_piece<T, DP>(v_tile, here, t), go[t], dp);
+        s = multiply<T>(row_piece<T, DP>(k_tile, here, t), q[t], s);
+        dp = multiply<T>(row_piece<T, DP>(v_tile, here, t), go[t], dp);
       }
       float ds[16];
       const float low = delta * scaled.power;
@@ -1008,31 +1089,16 @@ template <typename T, int DP> struct StatesShape {
 // all kKeys tile rows in their order.
 template <typename T, int DP, int KEYS>
 __device__ inline f32x16 accumulate_rows(const char* tile, int block, const char* scores, int row, f32x16 acc) {
-  const int lane = threadIdx.x % kWave, half = lane / 32;
+  const int half = int(threadIdx.x % kWave) / 32;
 #pragma unroll
-  for (int t = 0; t < Tile<T, KEYS>::kPieces / 2; ++t) {
-    const u32x4 b = row_piece<T, KEYS>(scores, row, t);
-    if constexpr (sizeof(T) == 2) {
-      const int channel = 32 * block + 16 * ((lane / 16) & 1) + 4 * (lane % 4);
-      i16x4 part[2];
+  for (int t = 0; t < KEYS / 16; ++t) {
+    typename Mma<T>::Vec a[Mma<T>::kPlanes], b[Mma<T>::kPlanes];
+    const auto piece = row_piece<T, KEYS>(scores, row, t);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int key = 16 * t + 8 * half + 4 * u + (lane % 16) / 4;
-        part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(
-            tile + Tile<T, DP>::offset(key, channel / 8) + (channel % 8) * 2));
-      }
-      const i16x8 both = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
-      acc = Mma<T>::mma(__builtin_bit_cast(typename Mma<T>::Vec, both), __builtin_bit_cast(typename Mma<T>::Vec, b), acc);
-    } else {
-      const int channel = 32 * block + lane % 32;
-      const f32x4 y = __builtin_bit_cast(f32x4, b);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = 8 * t + 4 * half + i;
-        const float x = *reinterpret_cast<const float*>(tile + Tile<T, DP>::offset(key, channel / 4) + (channel % 4) * 4);
-        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x, y[i], acc, 0, 0, 0);
-      }
-    }
+    for (int p = 0; p < Mma<T>::kPlanes; ++p) b[p] = __builtin_bit_cast(typename Mma<T>::Vec, piece.plane[p]);
+    const int key = 16 * t + 8 * half;
+    turned<T, DP>(tile, key, key + 4, block, a);
+    acc = Mma<T>::product(a, b, acc);
   }
   return acc;
 }
@@ -1128,25 +1194,26 @@ __global__ __launch_bounds__(kThreads, grad_states_waves(sizeof(T), DP, MASK, FU
   };
   if (first < last) load();
 
-  u32x4 k[kSteps], v[kSteps];
-  {
-    const T* k_row = static_cast<const T*>(a.k.at) + b * a.k.batch + int64_t(key) * a.k.row + kv * a.k.head;
-    const T* v_row = static_cast<const T*>(a.v.at) + b * a.v.batch + int64_t(key) * a.v.row + kv * a.v.head;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int c = (2 * s + lane / 32) * N;
-      const u32x4 zero = {0, 0, 0, 0};
-      k[s] = on ? load_piece(k_row, c, a.Dp) : zero;
-      v[s] = on ? load_piece(v_row, c, a.Dp) : zero;
-    }
-  }
+  typename Mma<T>::Piece k[kSteps], v[kSteps];
+  take_rows<T, DP>(a, static_cast<const T*>(a.k.at) + b * a.k.batch + int64_t(key) * a.k.row + kv * a.k.head, on, k);
+  take_rows<T, DP>(a, static_cast<const T*>(a.v.at) + b * a.v.batch + int64_t(key) * a.v.row + kv * a.v.head, on, v);
 
   f32x16 grad_k[NB] = {}, grad_v[NB] = {};
   Scaled<T> scaled;
   const float factor = MASK == kFloatMask ? a.scale : a.scale * kLog2e;
   auto put_score = [&](int row, float v) __attribute__((always_inline)) {
     const int at = 32 * wave + lane % 32;
-    *reinterpret_cast<T*>(scores + Tile<T, Shape::kKeys>::offset(row, at / N) + (at % N) * int(sizeof(T))) = static_cast<T>(v);
+    auto put = [&](int plane, auto x) __attribute__((always_inline)) {
+      *reinterpret_cast<decltype(x)*>(scores + Tile<T, Shape::kKeys>::offset(row, at / 8, plane) + (at % 8) * 2) = x;
+    };
+    if constexpr (sizeof(T) == 2) {
+      put(0, static_cast<T>(v));
+    } else {
+      bf16_t parts[3];
+      Mma<T>::split(v, parts);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) put(p, parts[p]);
+    }
   };
   auto step = [&](int64_t tile, auto buffer) __attribute__((always_inline)) {
     char* q_tile = lds + decltype(buffer)::value * Shape::kBuffer;
@@ -1172,7 +1239,7 @@ __global__ __launch_bounds__(kThreads, grad_states_waves(sizeof(T), DP, MASK, FU
 #pragma unroll
         for (int j = 0; j < N; ++j) dot = fmaf(widen(x[j]), widen(y[j]), dot);
 #pragma unroll
-        for (int by = 1; by < TileT::kPieces; by *= 2) dot += __shfl_xor(dot, by);
+        for (int by = 1; by < Stage<T, DP, kRows>::kPieces; by *= 2) dot += __shfl_xor(dot, by);
         if (o_stage.piece(i) == 0) row_delta[o_stage.row(i)] = -dot;
       }
     }
@@ -1185,7 +1252,9 @@ __global__ __launch_bounds__(kThreads, grad_states_waves(sizeof(T), DP, MASK, FU
     __syncthreads();
     if (tile + 1 < last) load();
 
-#pragma unroll
+    // Two blocks of rows unrolled take more registers than they hide: as fast at 64 channels, 8 %
+    // slower at 96 (2 x 452 rows of 1,171 states, 32 heads).
+#pragma unroll 1
     for (int n = 0; n < Shape::RB; ++n) {
       const int local = 32 * n;
       float add[16];
@@ -1221,8 +1290,8 @@ __global__ __launch_bounds__(kThreads, grad_states_waves(sizeof(T), DP, MASK, FU
       }
 #pragma unroll
       for (int t = 0; t < kSteps; ++t) {
-        s = Mma<T>::rows(row_piece<T, DP>(q_tile, local, t), k[t], s);
-        dp = Mma<T>::rows(row_piece<T, DP>(go_tile, local, t), v[t], dp);
+        s = multiply<T>(row_piece<T, DP>(q_tile, local, t), k[t], s);
+        dp = multiply<T>(row_piece<T, DP>(go_tile, local, t), v[t], dp);
       }
       float p[16], ds[16];
 #pragma unroll

@@ -58,7 +58,7 @@ Plan plan_of(const deformops_attention& c) {
     return int(std::max<int64_t>(1, std::min<int64_t>(kCus * waves / std::max<int64_t>(1, groups), tiles / 2)));
   };
   // The LDS of a workgroup whose waves share the rows (ForwardShape), in KB of a CU's 160.
-  const int tile = DP * size / 8, lds = 4 * tile <= 80 ? 4 * tile : std::max(2 * tile, DP / 2 + 1);
+  const int tile = DP * (size == 4 ? 6 : 2) / 8, lds = 4 * tile <= 80 ? 4 * tile : std::max(2 * tile, DP / 2 + 1);
   const int lds_waves = p.variant.few_rows ? 160 / lds : 4;
   p.splits = pieces(groups, std::min(lds_waves, forward_waves(size, DP, c.mask_kind)), tiles);
   p.variant.fused = c.keys > 0 && c.keys <= 128 && fused_shape(c.dtype == MSDA_F16, size, DP);
