@@ -257,6 +257,25 @@ def test_a_mask_of_states_leaves_them_unread(device, dtype):
 
 @pytest.mark.parametrize("device", BACKENDS)
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=IDS.get)
+@pytest.mark.parametrize("channels", [32, 64, 96])
+@pytest.mark.parametrize("states", [33, 100, 128])
+def test_masked_states_may_hold_anything_with_few_states(device, dtype, channels, states):
+    """At most 128 states: all gradients come from one pass, dq from the masked columns too."""
+    q, k, v, grad = tensors(2, 40, states, 4, 2, channels, dtype, on(device))
+    mask = torch.ones(2, 1, 1, states, dtype=torch.bool, device=device)
+    mask[0, ..., ::3] = mask[1, ..., 5:] = False
+    gone = ~mask[:, 0, 0]
+    k[gone], v[gone] = math.nan, -math.inf
+    got = run_and_check(q, k, v, mask=mask, grad=grad)
+    assert got["k"][gone].eq(0).all() and got["v"][gone].eq(0).all()
+    # Only the values, so that the scores stay finite.
+    k[gone] = 1
+    got = run_and_check(q, k, v, mask=mask, grad=grad)
+    assert got["k"][gone].eq(0).all() and got["v"][gone].eq(0).all()
+
+
+@pytest.mark.parametrize("device", BACKENDS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=IDS.get)
 def test_layouts(device, dtype):
     """Heads first, a packed projection, a batch that is one tensor for all, odd offsets."""
     q, k, v, grad = tensors(2, 50, 90, 4, 4, 24, dtype, on(device))
