@@ -128,6 +128,12 @@ variable_list once(variable_list out, const Tensor& grad) {
 // ---------------------------------------------------------------------------
 // Cross attention.
 
+// Dense and aligned to 16 bytes, as the backward reads it: a gradient may be a slice of another.
+Tensor dense(const Tensor& t) {
+  const Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
+
 // Channels side by side: any other layout is copied.
 Tensor rows(const Tensor& t) { return t.stride(3) == 1 || t.size(3) == 1 ? t : t.contiguous(); }
 
@@ -213,7 +219,7 @@ std::tuple<Tensor, Tensor, Tensor> attention_backward(const Tensor& q, const Ten
                                                       const Tensor& stats_in, const Tensor& grad_in) {
   const c10::OptionalDeviceGuard guard(q.device());
   Attention a(q, k, v, mask, lengths, scale);
-  const Tensor grad = grad_in.to(q.scalar_type()).contiguous(), out = out_in.contiguous(), stats = stats_in.contiguous();
+  const Tensor grad = dense(grad_in.to(q.scalar_type())), out = dense(out_in), stats = dense(stats_in);
   const at::DimVector expected = {a.call.batch, a.call.queries, a.call.heads * a.call.channels};
   TORCH_CHECK(grad.sizes() == expected && out.sizes() == expected && out.scalar_type() == q.scalar_type() &&
                   stats.scalar_type() == at::kFloat && stats.numel() == 2 * a.call.batch * a.call.heads * a.call.queries &&

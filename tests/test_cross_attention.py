@@ -225,6 +225,55 @@ def test_masks(device, sizes, kind, dtype):
         assert got["out"][:, ::step].eq(0).all() and got["q"][:, ::step].eq(0).all()
 
 
+def laid_out(mask: Tensor, layout: str) -> Tensor:
+    """The mask's values in another place: every second key of a wider row, keys first, or one
+    element past an aligned address."""
+    if layout == "second":
+        return mask.repeat_interleave(2, -1)[..., ::2]
+    if layout == "turned":
+        return mask.transpose(2, 3).contiguous().transpose(2, 3)
+    return mask.new_zeros(mask.numel() + 1)[1:].view(mask.shape).copy_(mask)
+
+
+@pytest.mark.parametrize("device", BACKENDS)
+@pytest.mark.parametrize("kind", ["bool", "float", "float16", "floatbf16"])
+@pytest.mark.parametrize("layout", ["second", "turned", "odd"])
+@pytest.mark.parametrize("states", [1, 2, 3, 4, 35, 130])
+def test_masks_in_other_layouts(device, kind, layout, states):
+    q, k, v, grad = tensors(2, 11, states, 4, 2, 24, BF16, on(device))
+    mask = make_mask(kind, 2, 4, 11, states, device)
+    expected = run_and_check(q, k, v, mask=mask, grad=grad)
+    got = run_and_check(q, k, v, mask=laid_out(mask, layout), grad=grad)
+    for name in got:
+        torch.testing.assert_close(got[name], expected[name], rtol=0, atol=0)
+
+
+@pytest.mark.parametrize("device", BACKENDS)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=IDS.get)
+@pytest.mark.parametrize("kind", ["none", "bool", "states", "float"])
+@pytest.mark.parametrize("channels", [20, 64, 128])
+def test_groups_of_heads_with_few_states(device, dtype, kind, channels):
+    """At most 128 states, in one pass; lengths beside the mask, one image without a state."""
+    q, k, v, grad = tensors(3, 150, 77, 6, 2, channels, dtype, on(device))
+    lengths = torch.tensor([77, 0, 33], device=device)
+    got = run_and_check(q, k, v, mask=make_mask(kind, 3, 6, 150, 77, device), lengths=lengths, grad=grad)
+    assert got["k"][1].eq(0).all() and got["q"][1].eq(0).all()
+
+
+@pytest.mark.parametrize("device", BACKENDS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=IDS.get)
+@pytest.mark.parametrize("states", [50, 200])
+def test_gradients_that_are_slices_of_others(device, dtype, states):
+    """torch.cat's gradient of the output is dense and starts one element past an aligned address."""
+    q, k, v, grad = tensors(2, 30, states, 4, 2, 32, dtype, on(device))
+    expected = run_and_check(q, k, v, grad=grad)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    together = torch.cat([grad.new_zeros(1), cross_attention(*leaves).flatten()])
+    got = torch.autograd.grad(together, leaves, torch.cat([grad.new_zeros(1), grad.flatten()]))
+    for a, b in zip(got, "qkv"):
+        torch.testing.assert_close(a, expected[b], rtol=0, atol=0)
+
+
 @pytest.mark.parametrize("device", BACKENDS)
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=IDS.get)
 @pytest.mark.parametrize("index", [torch.int32, torch.int64], ids=["i32", "i64"])
