@@ -24,10 +24,11 @@ bool rows_as_they_are(const deformops_attention& c, const void* p, const int64_t
 // Words of a bool mask's row: of whole tiles of 128 keys.
 int64_t mask_words(int64_t keys) { return ceil_div(keys, 128) * 4; }
 
-// Where one operand's packed copy lies in the workspace, if it has one.
+// Where one operand's packed copy lies in the workspace, if it has one, and the threads that
+// make it.
 struct Packed {
   bool on;
-  int64_t at;
+  int64_t at, threads;
 };
 
 struct Plan {
@@ -75,7 +76,8 @@ Plan plan_of(const deformops_attention& c) {
   };
   const int64_t Dp = ceil_div(c.channels, n) * n;
   auto pack = [&](bool as_it_is, int64_t rows_of, int64_t heads) {
-    return as_it_is ? Packed{false, 0} : Packed{true, take(c.batch * rows_of * heads * Dp * size)};
+    const int64_t elements = c.batch * rows_of * heads * Dp;
+    return as_it_is ? Packed{} : Packed{true, take(elements * size), elements / n};
   };
   p.q = pack(rows_as_they_are(c, c.query, c.query_strides, c.queries), c.queries, c.heads);
   p.k = pack(rows_as_they_are(c, c.key, c.key_strides, c.keys), c.keys, c.key_heads);
@@ -83,8 +85,9 @@ Plan plan_of(const deformops_attention& c) {
   const int64_t (&m)[4] = c.mask_strides;
   if (c.mask_kind != kNoMask && (c.mask_kind == kBoolMask || m[3] != 1 || c.keys < 4)) {
     const int64_t rows = (m[0] ? c.batch : 1) * (m[1] ? c.heads : 1) * (m[2] ? c.queries : 1);
-    p.mask = Packed{true, take(c.mask_kind == kBoolMask ? rows * mask_words(c.keys) * 4
-                                                        : rows * ceil_div(c.keys, 32) * 32 * element_size(c.mask_dtype))};
+    const bool bits = c.mask_kind == kBoolMask;
+    const int64_t threads = rows * (bits ? mask_words(c.keys) : ceil_div(c.keys, 32) * 32);
+    p.mask = Packed{true, take(threads * (bits ? 4 : element_size(c.mask_dtype))), threads};
   }
   // (The backward's sums of grad_q; none of them where that is fused.)
   p.part_at = take(p.splits > 1 ? p.splits * BK * R * c.channels * 4 : 0);
@@ -218,10 +221,17 @@ deformops_attention without_empty_mask(deformops_attention c) {
   return c;
 }
 
-int too_many(int64_t groups) {
-  return groups > (int64_t(1) << 31) - 1
+// Whether every launch of the call fits a grid: the walks' workgroups and the packed operands'.
+int too_many(const Plan& p, int64_t groups) {
+  for (const Packed* each : {&p.q, &p.k, &p.v, &p.o, &p.go, &p.mask})
+    if (each->on) groups = std::max(groups, ceil_div(each->threads, 256));
+  return groups > kMostGroups
              ? fail(MSDA_ERR_UNSUPPORTED, "cross attention: %lld workgroups pass a grid", static_cast<long long>(groups))
              : MSDA_OK;
+}
+
+int64_t row_groups(const deformops_attention& c, const Plan& p) {
+  return c.batch * c.key_heads * ceil_div(c.queries * (c.heads / c.key_heads), p.variant.few_rows ? 32 : 128) * p.splits;
 }
 
 }  // namespace
@@ -251,12 +261,12 @@ int deformops_cross_attention_forward(const deformops_attention* call, void* row
   if (p.forward_bytes && (!workspace || workspace_bytes < p.forward_bytes || !aligned(workspace, 256)))
     return fail(MSDA_ERR_INVALID, "cross attention: the workspace must hold %lld bytes, aligned to 256",
                 static_cast<long long>(p.forward_bytes));
+  const int64_t groups = row_groups(*c, p);
+  if (const int e = too_many(p, groups)) return e;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   Args a = args_of(*c, p, workspace, s);
   a.stats = static_cast<float2*>(row_stats);
   a.out_vector = a.D % 4 == 0 && aligned(c->output, 16);
-  const int64_t groups = int64_t(a.B) * a.K * ceil_div(a.R, p.variant.few_rows ? 32 : 128) * a.splits;
-  if (const int e = too_many(groups)) return e;
   with_type(c->dtype, [&](auto t) { launch_forward<decltype(t)>(a, c->mask_kind, p.variant, uint32_t(groups), s); });
   return launched("cross attention forward");
 }
@@ -278,6 +288,9 @@ int deformops_cross_attention_backward(const deformops_attention* call, const vo
   const int n = 16 / element_size(c->dtype);
   if (!aligned(c->output, 16) || !aligned(grad_output, 16))
     return fail(MSDA_ERR_INVALID, "cross attention: output and grad_output must be aligned to 16 bytes");
+  const int64_t groups = row_groups(*c, p);
+  const int64_t key_groups = c->batch * c->key_heads * ceil_div(c->keys, 128) * p.row_splits;
+  if (const int e = too_many(p, std::max(groups, key_groups))) return e;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   Args a = args_of(*c, p, workspace, s);
   const int64_t dense[3] = {c->queries * c->heads * c->channels, c->heads * c->channels, c->channels};
@@ -288,9 +301,6 @@ int deformops_cross_attention_backward(const deformops_attention* call, const vo
   a.grad_k = grad_key;
   a.grad_v = grad_value;
   a.out_vector = a.D % n == 0 && aligned(grad_query, 16) && aligned(grad_key, 16) && aligned(grad_value, 16);
-  const int64_t groups = int64_t(a.B) * a.K * ceil_div(a.R, p.variant.few_rows ? 32 : 128) * a.splits;
-  const int64_t key_groups = int64_t(a.B) * a.K * ceil_div(a.S, 128) * a.row_splits;
-  if (const int e = too_many(std::max(groups, key_groups))) return e;
   with_type(c->dtype, [&](auto t) {
     launch_backward<decltype(t)>(a, c->mask_kind, p.variant, uint32_t(groups), uint32_t(key_groups), s);
   });

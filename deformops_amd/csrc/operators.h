@@ -40,6 +40,9 @@ inline int launched(const char* what) {
   return e == hipSuccess ? MSDA_OK : fail(MSDA_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
 
+// Workgroups of 256 threads that one launch takes: fewer than 2^32 threads.
+constexpr int64_t kMostGroups = (int64_t(1) << 24) - 1;
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 inline bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }

@@ -187,7 +187,7 @@ extern "C" int deformops_rotary(const void* x, const int64_t* x_strides, void* y
   each = each < 1 ? 1 : each > 32 ? 32 : each;
   a.tokens = int(each < tokens ? each : tokens);
   a.groups_of_image = ceil_div(tokens, a.tokens);
-  if (a.groups_of_image * batch > (int64_t(1) << 31) - 1)
+  if (a.groups_of_image > kMostGroups / batch)
     return fail(MSDA_ERR_UNSUPPORTED, "rotary: the tokens pass a grid");
   const uint32_t groups = uint32_t(a.groups_of_image * batch);
   const hipStream_t s = static_cast<hipStream_t>(stream);
