@@ -87,8 +87,6 @@ def cross_attention_hip(query: Tensor, key: Tensor, value: Tensor, *, mask: Tens
                         key_lengths: Tensor | None = None, scale: float | None = None) -> Tensor:
     """Run cross attention on the gfx950 HIP kernels."""
     scale = default_scale(query.shape[3]) if scale is None else float(scale)
-    if mask is not None and mask.dtype == torch.float64:
-        mask = mask.to(torch.float32)
     if plain_eager(query, key, value, mask, key_lengths):
         return _native.load().cross_attention(query, key, value, mask, key_lengths, scale)
     return _forward_op(query, key, value, mask, key_lengths, scale)[0]

@@ -95,9 +95,9 @@ struct Args {
 // Matrix products of one wave.
 
 // Precision of a 16-bit operand made from fp32 scores: p and ds are rounded to the operands'
-// type (bf16 2^-9, f16 2^-12 relative). f16 has 5 exponent bits: the backward scales p by 2^14,
-// so that weights down to 2^-28 stay normal, and ds by a running power of two for each lane
-// (Scaled below). The forward's weights exp2(x - m) are scaled by 2^9.
+// type (by half a step: bf16 2^-8, f16 2^-11 relative). f16 has 5 exponent bits: the backward
+// scales p by 2^14, so that weights down to 2^-28 stay normal, and ds by a running power of
+// two for each lane (Scaled below). The forward's weights exp2(x - m) are scaled by 2^9.
 template <typename T> constexpr float kWeightBits = std::is_same_v<T, f16_t> ? 14.0f : 0.0f;
 template <typename T> constexpr float kForwardBits = std::is_same_v<T, f16_t> ? 9.0f : 0.0f;
 
