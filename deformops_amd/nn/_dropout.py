@@ -30,5 +30,8 @@ def drop_and_add(x: Tensor, p: float, *, training: bool, seed: int | Tensor | No
                 raise RuntimeError("dropout under graph capture needs seed, an int64 tensor that the graph reads at "
                                    "every replay")
             seed = int(torch.randint(2**63 - 1, ()))
+        if residual is not None and residual.dtype != x.dtype:  # as the sum without dropout
+            wide = torch.promote_types(x.dtype, residual.dtype)
+            x, residual = x.to(wide), residual.to(wide)
         return dropout(x, p, seed=seed, residual=residual, backend=backend)
     return x if residual is None else x + residual

@@ -83,6 +83,7 @@ class MultiScaleDeformAttn2d(nn.Module):
     """
 
     _version = 2
+    dropout: float = 0.0  # of layers that were pickled without one
 
     def __init__(
         self,

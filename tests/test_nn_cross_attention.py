@@ -153,6 +153,34 @@ def test_dropout_is_for_training_and_draws_its_seed():
     torch.testing.assert_close(layer(q, q, residual=q), layer(q, q) + q)
 
 
+@pytest.mark.parametrize("device", BACKENDS)
+@pytest.mark.parametrize("training", [True, False], ids=["train", "eval"])
+def test_a_residual_of_another_dtype(device, training):
+    """Under autocast the output is narrow and the residual is not: both are added in the wider dtype."""
+    torch.manual_seed(3)
+    layer = CrossAttention(32, num_heads=2, dropout=0.25).to(on(device)).train(training)
+    q = torch.randn(2, 9, 32, device=device)
+    residual = torch.randn(2, 9, 32, device=device, requires_grad=True)
+    with torch.autocast(device, dtype=BF16):
+        out = layer(q, q, residual=residual, seed=4)
+        bare = layer.eval()(q, q)
+    assert out.dtype == F32 and bare.dtype == BF16
+    wide = bare.float()
+    expected = dropout(wide, 0.25, seed=4, residual=residual) if training else wide + residual
+    assert torch.equal(out, expected)
+    grads = torch.autograd.grad(out.sum(), [residual, layer.proj_output.weight])
+    assert grads[0].eq(1).all() and grads[1].isfinite().all() and grads[1].ne(0).any()
+
+
+def test_an_msda_layer_that_was_pickled_without_dropout():
+    layer = MultiScaleDeformAttn2d(32, num_heads=4, num_levels=1)
+    inputs = (torch.randn(1, 3, 32), torch.rand(1, 3, 1, 2), torch.randn(1, 12, 32), torch.tensor([[4, 3]]),
+              torch.tensor([0]))
+    expected = layer(*inputs)
+    layer.__dict__.pop("dropout", None)
+    assert torch.equal(layer(*inputs), expected) and "dropout" not in repr(layer)
+
+
 @pytest.mark.gpu
 def test_a_captured_layer_needs_a_seed_in_memory(device):
     layer = CrossAttention(32, num_heads=2, dropout=0.5).to(device)
