@@ -6,7 +6,8 @@
 // backward is the same call on the gradient, without a residual.
 //
 // One thread makes a block's four words for four elements; the words cost 14 products of 32
-// bits for four elements. Bytes bound the large calls.
+// bits for four elements. Bytes bound the large calls: 88 million bf16 elements take 56 us, 6.3
+// TB/s read and written. Loads and stores pass the caches by, which such a stream only fills.
 
 #include <type_traits>
 
