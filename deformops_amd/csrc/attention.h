@@ -52,6 +52,8 @@ using namespace operators;
 
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef bf16_t bf16x2 __attribute__((ext_vector_type(2)));
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
 
@@ -166,6 +168,15 @@ template <> struct Mma<float> {
     out[1] = static_cast<bf16_t>(rest);
     out[2] = static_cast<bf16_t>(rest - static_cast<float>(out[1]));
   }
+  // The parts of x (the words' lower halves) and y: one conversion for both.
+  static __device__ void split(float x, float y, uint32_t (&out)[3]) {
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      out[p] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, bf16x2));
+      x -= __uint_as_float(out[p] << 16);
+      y -= __uint_as_float(out[p] & 0xffff0000u);
+    }
+  }
   static __device__ f32x16 product(const Vec (&a)[3], const Vec (&b)[3], f32x16 c) {
     c = Mma<bf16_t>::mma(a[2], b[0], c);  // the smallest first
     c = Mma<bf16_t>::mma(a[0], b[2], c);
@@ -175,26 +186,30 @@ template <> struct Mma<float> {
     return Mma<bf16_t>::mma(a[0], b[0], c);
   }
   static __device__ Weights weights(const float (&w)[16]) {
+    u32x4 words[2][3];
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      uint32_t parts[3];
+      split(w[i], w[i + 1], parts);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) words[i / 8][p][i % 8 / 2] = parts[p];
+    }
     Weights out;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      bf16_t parts[3];
-      split(w[i], parts);
-#pragma unroll
-      for (int p = 0; p < 3; ++p) out.part[i / 8][p][i % 8] = parts[p];
-    }
+    for (int p = 0; p < 6; ++p) out.part[p / 3][p % 3] = __builtin_bit_cast(Vec, words[p / 3][p % 3]);
     return out;
   }
   static __device__ Piece piece(const u32x4 (&memory)[2]) {
-    Vec out[3];
+    Piece out;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      bf16_t parts[3];
-      split(__builtin_bit_cast(f32x4, memory[i / 4])[i % 4], parts);
+    for (int i = 0; i < 8; i += 2) {
+      const f32x4 four = __builtin_bit_cast(f32x4, memory[i / 4]);
+      uint32_t parts[3];
+      split(four[i % 4], four[i % 4 + 1], parts);
 #pragma unroll
-      for (int p = 0; p < 3; ++p) out[p][i] = parts[p];
+      for (int p = 0; p < 3; ++p) out.plane[p][i / 2] = parts[p];
     }
-    return Piece{{__builtin_bit_cast(u32x4, out[0]), __builtin_bit_cast(u32x4, out[1]), __builtin_bit_cast(u32x4, out[2])}};
+    return out;
   }
 };
 
@@ -502,16 +517,14 @@ template <typename T, int DP, int ROWS> struct Stage {
       if constexpr (sizeof(T) == 2) {
         *reinterpret_cast<u32x4*>(tile + Tile<T, DP>::offset(row(i), piece(i))) = hold[i];
       } else {  // half a piece of each plane
-        bf16_t parts[4][3];
+        const f32x4 four = __builtin_bit_cast(f32x4, hold[i]);
+        uint32_t low[3], high[3];
+        Mma<T>::split(four[0], four[1], low);
+        Mma<T>::split(four[2], four[3], high);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) Mma<T>::split(__builtin_bit_cast(f32x4, hold[i])[j], parts[j]);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) {
-          const bf16_t four[4] = {parts[0][p], parts[1][p], parts[2][p], parts[3][p]};
-          u32x2 w;
-          __builtin_memcpy(&w, four, 8);
-          *reinterpret_cast<u32x2*>(tile + Tile<T, DP>::offset(row(i), piece(i) / 2, p) + 8 * (piece(i) % 2)) = w;
-        }
+        for (int p = 0; p < 3; ++p)
+          *reinterpret_cast<u32x2*>(tile + Tile<T, DP>::offset(row(i), piece(i) / 2, p) + 8 * (piece(i) % 2)) =
+              u32x2{low[p], high[p]};
       }
     }
   }
