@@ -5,6 +5,10 @@ A drop-in for deformops' MSDA operator on AMD Instinct MI355X (gfx950): the
 operators, backed by hand-written HIP kernels: a forward, and a backward that
 writes every element of ``grad_value`` once from fp32 registers (owner-computes,
 no atomics on the gradient and no buffer beyond the three gradients).
+
+Beside MSDA: ``registry.cross_attention``, ``registry.rotary`` and
+``registry.dropout``, which a decoder around it runs, and ``nn.CrossAttention``, the
+three as one layer.
 """
 
 from __future__ import annotations

@@ -29,6 +29,7 @@ __all__ = [
     "PATH_TILE8",
     "INDEX_CODES",
     "EXPORTED_SYMBOLS",
+    "OPERATOR_SYMBOLS",
     "Library",
     "library_path",
     "load",
@@ -56,7 +57,7 @@ PATH_NO_MFMA = 1
 PATH_ATOMIC_SORT = 2
 PATH_TILE8 = 4
 
-#: Every function the header declares.
+#: Every MSDA function the header declares.
 EXPORTED_SYMBOLS = (
     "msda_forward",
     "msda_backward",
@@ -69,6 +70,9 @@ EXPORTED_SYMBOLS = (
     "msda_record_plan",
     "msda_set_path_override",
     "msda_set_phase_events",
+)
+#: The functions of the operators beside it.
+OPERATOR_SYMBOLS = (
     "deformops_cross_attention_workspace_size",
     "deformops_cross_attention_forward",
     "deformops_cross_attention_backward",

@@ -34,7 +34,7 @@
 //   forward, and all gradients in one pass (FUSED), 2 x 21,504 rows of 77 states, 8 heads of 64, bf16:
 //     32 us, 2.7 TB/s, and 59 us, 3.0 TB/s, bound by the time a tile takes from its loads to its
 //     stores.
-//   4 x 100 rows of 16,384 states, 8 heads of 32, bf16, bool mask: forward 26 us, grad_q 34 us,
+//   4 x 100 rows of 16,384 states, 8 heads of 32, bf16, bool mask: forward 26 us, grad_q 33 us,
 //     2.5 and 2.0 TB/s, grad_states 49 us, 2.7 TB/s: the prologue and epilogue of short walks.
 
 #ifndef DEFORMOPS_AMD_ATTENTION_H_

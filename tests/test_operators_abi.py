@@ -4,6 +4,8 @@ and dropout. Nothing is launched: every call here ends at a check, or asks for s
 from __future__ import annotations
 
 import ctypes
+import re
+from pathlib import Path
 
 import pytest
 
@@ -52,6 +54,14 @@ def forward(lib, call, workspace=None, size=0):
 def backward(lib, call, workspace=None, size=0, grad=SOME, grads=(SOME, SOME, SOME), stats=SOME):
     return lib.deformops_cross_attention_backward(ctypes.byref(call), P(stats), P(grad), *(P(g) for g in grads),
                                                   P(workspace), L(size), None)
+
+
+def test_every_declared_function_is_exported_and_bound(lib):
+    header = Path(__file__).resolve().parents[1] / "include" / "deformops_amd.h"
+    declared = re.findall(r"^(?:int|const char\*)\s+(deformops_\w+)\(", header.read_text(), flags=re.M)
+    assert set(declared) == set(_lib.OPERATOR_SYMBOLS)
+    for name in declared:
+        assert getattr(lib, name).argtypes is not None
 
 
 def test_the_structure_is_the_headers(lib):
