@@ -107,12 +107,13 @@ def _cross_attention_call(
     Notes
     -----
     Scores, softmax and every sum are in float32. 16-bit products are exact in it;
-    float32 products are formed of three bfloat16 parts each, to 2^-23 of their size, and
-    an attended infinity gives NaN there. The weights and their gradients are rounded to a
-    16-bit operands' type before the second products. Equal calls give equal bits. States that ``key_lengths`` removes, or a
-    boolean mask of shape ``(.., 1, 1, S)``, may hold anything, NaN included; states
-    that a mask removes from some queries only, or a floating mask removes, must be
-    finite, as in the formula.
+    float32 products are formed on the GPU of three bfloat16 parts each, to 2^-23 of
+    their size, and an attended infinity, or a value past bfloat16's range (3.39e38),
+    gives NaN there. The weights and their gradients are rounded to a 16-bit operands'
+    type before the second products. Equal calls give equal bits. States that
+    ``key_lengths`` removes, or a boolean mask of shape ``(.., 1, 1, S)``, may hold
+    anything, NaN included; states that a mask removes from some queries only, or a
+    floating mask removes, must be finite, as in the formula.
     """
     raise NotImplementedError
 
